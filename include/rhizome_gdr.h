@@ -75,7 +75,9 @@ const char *rhz_last_error(void);
  * host-buffer scan, the device status query and the chunked-form setting;
  * 2.0 gives the bf16 tensor-core path caller-owned scratch: a workspace
  * argument on rhz_gdr_varlen_fwd(_norm), and rhz_gdr_workspace_bytes takes
- * the head count, width and dtype. */
+ * the head count, width and dtype. Entries added since then (the Global
+ * blocks' attention and cache, rhz_gdr_tree_step) change no earlier one and
+ * keep the number. */
 #define RHZ_ABI_VERSION 200
 int rhz_abi_version(void);
 
@@ -277,6 +279,34 @@ int rhz_gdr_multistep(void *outs, float *states, const float *state_pool,
                       int32_t dtype, rhz_stream_t stream);
 
 /*
+ * rhz_gdr_tree_step -- rhz_gdr_multistep over trees of drafted tokens, an
+ * addition of this library (the reference scores chains only,
+ * gated_delta_multistep, crates/ops/src/delta.rs:201-230). Sequence i's nodes
+ * are the packed rows [cu_seqlens[i], cu_seqlens[i+1]) of q/k/v/alpha/beta;
+ * parent[row] is the index of the node's parent within its own sequence, -1
+ * for a child of the sequence's committed state, and comes before the node
+ * (parent == NULL: every node's parent is the one before it). Node t gets
+ *   S_t = alpha_t (S_p - beta_t (S_p k_t) k_t^T) + beta_t v_t k_t^T, o_t = S_t q_t
+ * from its parent's state S_p, or from state_pool[slot_idx[i]] (slot i when
+ * slot_idx is NULL; zeros when state_pool is NULL). Writes o [tokens][H][d]
+ * and states [tokens][H][d][d] f32; the pool is not modified. The state of
+ * the last accepted node is committed afterwards (e.g. with
+ * rhz_varlen_scatter_states). A node whose parent is neither -1 nor an
+ * earlier node that takes part, and every node past the first max_positions
+ * (at most 64) of its sequence, takes no part: its row of o is zero and its
+ * states are left as they were (a fixed-size batch marks its padding with
+ * parent -2). Rows past cu_seqlens[n_seq] are left as they were. A slot index
+ * outside [0, num_slots) starts from zeros and writes NaN to the sequence's
+ * rows of o.
+ */
+int rhz_gdr_tree_step(void *o, float *states, const float *state_pool, const int32_t *slot_idx,
+                      const int32_t *cu_seqlens, const int32_t *parent, const void *q,
+                      const void *k, const void *v, const float *alpha, const float *beta,
+                      int64_t n_seq, int64_t total_tokens, int64_t max_positions,
+                      int64_t num_slots, int32_t H, int32_t d, int32_t dtype,
+                      rhz_stream_t stream);
+
+/*
  * rhz_gdr_prep -- the Local block's input producer (SPEC.md:53-54, 61-63),
  * the step in front of the recurrence, built from the reference's pieces:
  * per channel the causal depthwise conv of kernel 4, causal_conv1d_step
@@ -343,6 +373,120 @@ size_t rhz_gdr_bwd_workspace_bytes(int64_t B, int64_t T, int32_t H, int32_t d);
  */
 size_t rhz_gdr_workspace_bytes(int64_t B, int64_t T, int32_t H, int32_t d, int32_t dtype,
                                int has_segment);
+
+/* --------------------------------------------------------------------- */
+/* Softmax attention of the Global blocks, and its paged cache             */
+/* --------------------------------------------------------------------- */
+
+/*
+ * Every sixth block of the trunk is a Global block (crates/ops/src/
+ * attention.rs: mla_prefill :164, mla_decode :226); these entries give it
+ * the serving forms that the Local blocks have above: a packed prefill, and
+ * single tokens or drafted trees over what a sequence keeps, with K and V per
+ * (grouped) head. The reference caches positions contiguously; here they live
+ * in pages:
+ *   k_cache, v_cache  [num_blocks][H_kv][page][d]   dtype
+ *   block_table       [n][width] int32: page p of request i holds its
+ *                     positions [p * page, (p + 1) * page); entries outside
+ *                     [0, num_blocks) have no memory behind them
+ *   slot              block * page + position % page (int64), -1 for none
+ * page is a power of two, 8 to 1024.
+ */
+
+/*
+ * rhz_kv_step_tables -- what one engine step needs to address the cache, from
+ * request lengths, without a round trip to the host. Request i has cached[i]
+ * positions in the cache, owns the first held[i] entries of its table row,
+ * and adds fresh[i] positions in this step (negative lengths count as 0). Its
+ * missing pages, need_i = max(0, min(ceil((cached_i + fresh_i) / page),
+ * width) - held_i) if fresh_i > 0, are taken in request order from
+ * free_blocks[*cursor ..num_free) (cursor NULL: from its start). Writes
+ *   cu_seqlens [n + 1]   prefix sums of fresh (their total below 2^31)
+ *   block_table          the new entries only; others stay as they are
+ *   held_out [n]         pages owned now
+ *   cursor_out [1]       the cursor past the pages taken
+ *   missing [1]          pages that were needed and not to be had, because
+ *                        the free list or the table's width ended
+ *   slot_map [max_tokens] the slot of every packed row; -1 for rows whose page
+ *                        is missing and for rows past the total
+ * all int32 but slot_map. held_out and cursor_out must not be held and
+ * cursor themselves (copy them back, or alternate two sets).
+ */
+int rhz_kv_step_tables(int32_t *cu_seqlens, int64_t *slot_map, int32_t *block_table,
+                       int32_t *held_out, int32_t *cursor_out, int32_t *missing,
+                       const int32_t *cached, const int32_t *fresh, const int32_t *held,
+                       const int32_t *free_blocks, const int32_t *cursor, int64_t n,
+                       int64_t width, int64_t num_free, int64_t max_tokens, int32_t page,
+                       rhz_stream_t stream);
+
+/*
+ * rhz_kv_append -- K and V rows into the cache: row t of k and v ([H_kv][d],
+ * rows k_stride and v_stride elements apart, so slices of a fused projection
+ * will do) goes to slot slot_map[t]; rows whose slot is outside
+ * [0, num_blocks * page) are skipped. Slots must be distinct. Appending the
+ * accepted rows of a drafted tree again, at their final slots (-1 for the
+ * others), closes the gaps that the rejected ones leave. d a multiple of 4,
+ * at most 256; strides multiples of 4; caches 16-byte, k and v 8-byte (bf16)
+ * or 16-byte (f32) aligned.
+ */
+int rhz_kv_append(void *k_cache, void *v_cache, const void *k, const void *v,
+                  const int64_t *slot_map, int64_t tokens, int64_t k_stride, int64_t v_stride,
+                  int64_t num_blocks, int32_t page, int32_t H_kv, int32_t d, int32_t dtype,
+                  rhz_stream_t stream);
+
+/*
+ * rhz_attn_varlen_fwd -- causal softmax attention over packed prompts, beside
+ * rhz_gdr_varlen_fwd on the same stream of tokens. Query head h reads K/V
+ * head h / (H / H_kv). For row t of a sequence, over its rows j <= t:
+ *   s_j = scale q_t . k_j,  o_t = sum_j exp(s_j) v_j / sum_j exp(s_j),
+ *   lse_t = log sum_j exp(s_j)
+ * q [tokens][H][d], k and v [tokens][H_kv][d], rows q_stride, k_stride,
+ * v_stride elements apart (multiples of 8 for bf16, 4 for f32, 16-byte
+ * aligned bases); o [tokens][H][d] contiguous; lse [tokens][H] f32 or NULL.
+ * Rows outside [cu_seqlens[0], cu_seqlens[n_seq]) are left as they were.
+ * Values of rows that a row does not see never reach it, NaN and infinities
+ * included. H a multiple of H_kv, at most 64 query heads to a K/V head; d a
+ * multiple of 4 (8 for bf16), at most 256; scale finite and positive.
+ * bf16 with d of 64 or 128 runs on the tensor cores (products of bf16 with
+ * f32 sums, probabilities rounded to bf16), everything else in f32
+ * arithmetic. Results do not depend on what else is in the batch.
+ */
+int rhz_attn_varlen_fwd(void *o, float *lse, const void *q, const void *k, const void *v,
+                        const int32_t *cu_seqlens, int64_t n_seq, int64_t total_tokens,
+                        int64_t q_stride, int64_t k_stride, int64_t v_stride, int32_t H,
+                        int32_t H_kv, int32_t d, float scale, int32_t dtype,
+                        rhz_stream_t stream);
+
+/*
+ * rhz_attn_tree_fwd -- the same attention for drafted trees (or single
+ * tokens) over the paged cache, beside rhz_gdr_tree_step and rhz_gdr_step.
+ * Sequence i's query rows [cu_seqlens[i], cu_seqlens[i+1]) are its drafted
+ * nodes, whose own K and V rhz_kv_append has put at positions cached[i] + t.
+ * Node t sees the cached[i] positions before and, of the nodes, itself and
+ * its ancestors by `parent` (as in rhz_gdr_tree_step; NULL: every node up to
+ * itself, i.e. plain decode with one node, or a further piece of a prompt).
+ * With a parent array a sequence has at most 64 nodes: max_positions bounds
+ * the nodes that take part (at most 64 with `parent`), and the choice of form
+ * goes by it, so pass the engine's own bound. Nodes that take no part, by
+ * the bound or by their parent, or whose own position is beyond the table,
+ * see nothing: o = 0, lse = -inf. Positions whose table entry is outside
+ * [0, num_blocks) are seen by nobody. Rows outside [cu_seqlens[0],
+ * cu_seqlens[n_seq]) are left as they were. The key axis of a sequence is
+ * computed in chunks chosen by its own length and joined in order, so results
+ * do not depend on the batch; `workspace` holds
+ * rhz_attn_tree_workspace_bytes(...) bytes (256-byte aligned; NULL/0 when
+ * that is 0); calls that share a workspace must not overlap on the GPU.
+ */
+int rhz_attn_tree_fwd(void *o, float *lse, const void *q, const void *k_cache,
+                      const void *v_cache, const int32_t *block_table, const int32_t *cached,
+                      const int32_t *cu_seqlens, const int32_t *parent, int64_t n_seq,
+                      int64_t total_tokens, int64_t max_positions, int64_t q_stride,
+                      int64_t width, int64_t num_blocks, int32_t page, int32_t H, int32_t H_kv,
+                      int32_t d, float scale, int32_t dtype, void *workspace,
+                      size_t workspace_bytes, rhz_stream_t stream);
+size_t rhz_attn_tree_workspace_bytes(int64_t total_tokens, int64_t max_positions, int64_t width,
+                                     int32_t page, int32_t H, int32_t H_kv, int32_t d,
+                                     int32_t dtype);
 
 /* --------------------------------------------------------------------- */
 /* Variable-length packing (bit-exact index work)                         */

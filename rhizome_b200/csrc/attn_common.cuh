@@ -1,0 +1,145 @@
+// What the attention kernels share: which keys a row sees, how the key axis
+// of a paged sequence is split, and where partial results go.
+//
+// Rows. A (sequence, K/V head) pair's query rows are ordered (token, head of
+// the group): row r is token r / G, query head g * G + r % G, G = H / Hkv, so
+// the rows of a tile share every K and V tile they read and a short sequence
+// still fills tiles when the group is large.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace rhz {
+namespace attn {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int MAX_NODES = 64;  // drafted tokens of one sequence (one bit each)
+
+// Splitting the key axis. A paged sequence of L keys is cut into chunks of
+// span(L) keys, anchored at its first key, each computed by itself and joined
+// afterwards in order of position. The rule looks at this sequence's length
+// alone, so a sequence's result does not depend on what else is in the batch.
+struct Split {
+    int least;  // keys per chunk at least (a multiple of 128)
+    int most;   // chunks per sequence at most
+    __host__ __device__ int64_t span(int64_t L) const {
+        int64_t c = (L + most - 1) / most;
+        c = (c + 127) / 128 * 128;
+        return c < least ? least : c;
+    }
+    __host__ __device__ int64_t chunks(int64_t L) const {
+        const int64_t c = span(L);
+        return L <= 0 ? 1 : (L + c - 1) / c;
+    }
+    // The most chunks that any length up to L can have.
+    int64_t bound(int64_t L) const {
+        const int64_t c = (L + least - 1) / least;
+        return c < 1 ? 1 : (c < most ? c : most);
+    }
+};
+
+// Partial results in the workspace: chunk counts [tokens], then log-sum-exp
+// (base 2) [chunk][tokens][H], then normalised outputs [chunk][tokens][H][d].
+struct Parts {
+    int32_t *count;
+    float *lse, *o;
+    int64_t tokens;
+    int H, d, most;  // most: chunks that the workspace has room for
+    __device__ int64_t row(int64_t c, int64_t token, int head) const {
+        return (c * tokens + token) * H + head;
+    }
+};
+
+inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+inline size_t parts_bytes(int64_t tokens, int H, int d, int64_t chunks) {
+    if (chunks <= 1 || tokens <= 0) return 0;
+    const size_t rows = static_cast<size_t>(chunks) * tokens * H;
+    return up256(tokens * sizeof(int32_t)) + up256(rows * sizeof(float)) + rows * d * sizeof(float);
+}
+
+inline Parts parts_at(void *ws, int64_t tokens, int H, int d, int64_t chunks) {
+    Parts p{};
+    p.tokens = tokens;
+    p.H = H;
+    p.d = d;
+    p.most = static_cast<int>(chunks);
+    if (chunks <= 1 || ws == nullptr) return p;
+    char *b = static_cast<char *>(ws);
+    const size_t rows = static_cast<size_t>(chunks) * tokens * H;
+    p.count = reinterpret_cast<int32_t *>(b);
+    p.lse = reinterpret_cast<float *>(b + up256(tokens * sizeof(int32_t)));
+    p.o = reinterpret_cast<float *>(b + up256(tokens * sizeof(int32_t)) + up256(rows * sizeof(float)));
+    return p;
+}
+
+// One sequence as the kernels see it: offsets clamped to the buffers, so that
+// no cu_seqlens, length or table can lead outside them.
+struct Seq {
+    int64_t first;   // first query row
+    int64_t m;       // query rows
+    int64_t live;    // of which take part (m, at most `most`)
+    int64_t cached;  // keys before the sequence's own rows (0 packed)
+    int64_t keys;    // cached + live
+};
+
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int64_t i) {
+    Seq s;
+    s.first = min(max(static_cast<int64_t>(a.cu_seqlens[i]), int64_t{0}), a.total_tokens);
+    s.m = min(max(static_cast<int64_t>(a.cu_seqlens[i + 1]), s.first), a.total_tokens) - s.first;
+    s.cached = 0;
+    s.live = s.m;
+    if (a.paged) {
+        const int64_t room = a.width << a.shift;
+        s.live = min(s.m, a.most);
+        s.cached = min(max(static_cast<int64_t>(a.cached[i]), int64_t{0}), room);
+        s.live = min(s.live, room - s.cached);  // rows whose own key has no table entry take no part
+    }
+    s.keys = s.cached + s.live;
+    return s;
+}
+
+// Ancestors of drafted token t, itself included, as bits; 0 where t takes no
+// part: its parent is not -1 or an earlier token, or some ancestor's is not.
+__device__ __forceinline__ uint64_t ancestors(const int32_t *parent, int64_t t) {
+    uint64_t bits = 0;
+    int64_t p = t;
+    while (p >= 0) {
+        bits |= uint64_t{1} << p;
+        const int64_t up = parent[p];
+        if (up < -1 || up >= p) return 0;
+        p = up;
+    }
+    return bits;
+}
+
+// The keys that one row sees: all below `all`, and of the 64 from `all` on
+// those whose bit is set.
+struct Sight {
+    int64_t all;
+    uint64_t bits;
+    __device__ __forceinline__ bool sees(int64_t key) const {
+        if (key < all) return true;
+        const int64_t b = key - all;
+        return b < 64 && (bits >> b & 1);
+    }
+};
+
+__device__ __forceinline__ Sight sight_of(const AttnArgs &a, const Seq &s, int64_t t) {
+    if (t >= s.live) return {0, 0};
+    if (a.paged && a.parent) {
+        const uint64_t bits = ancestors(a.parent + s.first, t);
+        return {bits ? s.cached : 0, bits};
+    }
+    return {s.cached + t + 1, 0};
+}
+
+}  // namespace attn
+}  // namespace rhz

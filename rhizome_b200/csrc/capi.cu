@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -242,13 +243,14 @@ int rhz_abi_version(void) { return RHZ_ABI_VERSION; }
 int rhz_device_status(int32_t *timed_out, int clear) {
     clear_error();
     if (!timed_out) return set_error(RHZ_ERR_INVALID, "timed_out must not be NULL");
-    int a = 0, b = 0, c = 0, e = 0;
+    int a = 0, b = 0, c = 0, e = 0, f = 0;
     int st = chunk_pair_status(&a, clear != 0);
     if (st == RHZ_OK) st = chunk_solo_status(&b, clear != 0);
     if (st == RHZ_OK) st = chunk_grid_status(&c, clear != 0);
     if (st == RHZ_OK) st = prep_status(&e, clear != 0);
+    if (st == RHZ_OK) st = attn_status(&f, clear != 0);
     if (st != RHZ_OK) return st;
-    *timed_out = (a | b | c | e) ? 1 : 0;
+    *timed_out = (a | b | c | e | f) ? 1 : 0;
     return RHZ_OK;
 }
 
@@ -602,6 +604,41 @@ int rhz_gdr_multistep(void *outs, float *states, const float *state_pool,
     return launch_multistep(a);
 }
 
+int rhz_gdr_tree_step(void *o, float *states, const float *state_pool, const int32_t *slot_idx,
+                      const int32_t *cu_seqlens, const int32_t *parent, const void *q,
+                      const void *k, const void *v, const float *alpha, const float *beta,
+                      int64_t n_seq, int64_t total_tokens, int64_t max_positions,
+                      int64_t num_slots, int32_t H, int32_t d, int32_t dtype,
+                      rhz_stream_t stream) {
+    clear_error();
+    RHZ_TRY(check_dtype(dtype));
+    RHZ_TRY(check_heads(H, d));
+    if (n_seq < 0 || total_tokens < 0 || max_positions < 0 || num_slots < 0)
+        return set_error(RHZ_ERR_SHAPE, "negative size (n_seq %lld, total_tokens %lld, max_positions %lld, num_slots %lld)",
+                         (long long)n_seq, (long long)total_tokens, (long long)max_positions, (long long)num_slots);
+    if (max_positions > 64) return set_error(RHZ_ERR_SHAPE, "a drafted tree has at most 64 positions (got %lld)", (long long)max_positions);
+    if (state_pool && slot_idx == nullptr && n_seq > num_slots)
+        return set_error(RHZ_ERR_SHAPE, "n_seq = %lld sequences but only %lld slots (slot_idx is NULL)", (long long)n_seq, (long long)num_slots);
+    if (n_seq * H > INT32_MAX || total_tokens > INT32_MAX)
+        return set_error(RHZ_ERR_SHAPE, "n_seq*H = %lld or total_tokens = %lld exceeds int32 indexing", (long long)(n_seq * H), (long long)total_tokens);
+    if (n_seq == 0 || total_tokens == 0) return RHZ_OK;
+    RHZ_TRY(check_ptr(q, "q", 16, true));
+    RHZ_TRY(check_ptr(k, "k", 16, true));
+    RHZ_TRY(check_ptr(v, "v", 16, true));
+    RHZ_TRY(check_ptr(o, "o", 16, true));
+    RHZ_TRY(check_ptr(states, "states", 16, true));
+    RHZ_TRY(check_ptr(alpha, "alpha", 4, true));
+    RHZ_TRY(check_ptr(beta, "beta", 4, true));
+    RHZ_TRY(check_ptr(cu_seqlens, "cu_seqlens", 4, true));
+    RHZ_TRY(check_ptr(parent, "parent", 4, parent != nullptr));
+    RHZ_TRY(check_ptr(state_pool, "state_pool", 16, state_pool != nullptr));
+    RHZ_TRY(check_ptr(slot_idx, "slot_idx", 4, slot_idx != nullptr));
+    RHZ_TRY(require_sm100());
+    TreeArgs a{o, states, state_pool, slot_idx, cu_seqlens, parent, q, k, v, alpha, beta, n_seq,
+               total_tokens, static_cast<int>(max_positions), num_slots, H, d, dtype, as_cuda(stream)};
+    return launch_tree(a);
+}
+
 int rhz_gdr_prep(void *q, void *k, void *v, float *alpha, float *beta, const void *xq,
                  const void *xk, const void *xv, const float *beta_logit, const float *alpha_logit,
                  const float *a_head, const float *conv_w, const float *conv_b, float *conv_state,
@@ -952,6 +989,225 @@ int rhz_gdr_scan_chunked_host(void *o, float *state_final, const void *q, const 
     if (e == cudaSuccess) e = e2 != cudaSuccess ? e2 : e3;
     if (e != cudaSuccess) return set_error(RHZ_ERR_DEVICE, "host-buffer scan: %s", cudaGetErrorString(e));
     return RHZ_OK;
+}
+
+}  // extern "C"
+
+// ---- softmax attention and its paged cache
+
+namespace {
+
+// log2 of a page size, or the error.
+int check_page(int32_t page, int *shift) {
+    for (int s = 3; s <= 10; ++s)
+        if (page == 1 << s) {
+            *shift = s;
+            return RHZ_OK;
+        }
+    return set_error(RHZ_ERR_SHAPE, "page = %d: a power of two, 8 to 1024", page);
+}
+
+int check_attn_heads(int32_t H, int32_t H_kv, int32_t d, int32_t dtype) {
+    RHZ_TRY(check_dtype(dtype));
+    RHZ_TRY(check_heads(H, d));
+    if (H_kv < 1 || H % H_kv)
+        return set_error(RHZ_ERR_SHAPE, "H = %d query heads do not split evenly over H_kv = %d", H, H_kv);
+    if (H / H_kv > 64)
+        return set_error(RHZ_ERR_SHAPE, "%d query heads to a K/V head: at most 64", H / H_kv);
+    const int unit = dtype == RHZ_DTYPE_BF16 ? 8 : 4;
+    if (d % unit) return set_error(RHZ_ERR_SHAPE, "head_dim = %d: a multiple of %d for this dtype", d, unit);
+    return RHZ_OK;
+}
+
+int check_scale(float scale) {
+    if (!(scale > 0.f) || !(scale < INFINITY))
+        return set_error(RHZ_ERR_INVALID, "scale = %g: must be finite and positive", (double)scale);
+    return RHZ_OK;
+}
+
+int check_stride(int64_t stride, int64_t row, int32_t dtype, const char *name) {
+    const int unit = dtype == RHZ_DTYPE_BF16 ? 8 : 4;
+    if (stride < row || stride % unit || stride > (int64_t{1} << 36))
+        return set_error(RHZ_ERR_SHAPE, "%s = %lld: at least %lld and a multiple of %d", name, (long long)stride, (long long)row, unit);
+    return RHZ_OK;
+}
+
+int check_attn_sizes(int64_t n_seq, int64_t total_tokens, int32_t H) {
+    if (n_seq < 0 || total_tokens < 0)
+        return set_error(RHZ_ERR_SHAPE, "negative size (n_seq %lld, total_tokens %lld)", (long long)n_seq, (long long)total_tokens);
+    if (n_seq > INT32_MAX - 1 || total_tokens > INT32_MAX - 1 || total_tokens * H > (int64_t{1} << 33))
+        return set_error(RHZ_ERR_SHAPE, "n_seq = %lld, total_tokens = %lld: beyond int32 indexing", (long long)n_seq, (long long)total_tokens);
+    return RHZ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rhz_kv_step_tables(int32_t *cu_seqlens, int64_t *slot_map, int32_t *block_table,
+                       int32_t *held_out, int32_t *cursor_out, int32_t *missing,
+                       const int32_t *cached, const int32_t *fresh, const int32_t *held,
+                       const int32_t *free_blocks, const int32_t *cursor, int64_t n,
+                       int64_t width, int64_t num_free, int64_t max_tokens, int32_t page,
+                       rhz_stream_t stream) {
+    clear_error();
+    int shift = 0;
+    RHZ_TRY(check_page(page, &shift));
+    if (n < 0 || width < 0 || num_free < 0 || max_tokens < 0)
+        return set_error(RHZ_ERR_SHAPE, "negative size (n %lld, width %lld, num_free %lld, max_tokens %lld)",
+                         (long long)n, (long long)width, (long long)num_free, (long long)max_tokens);
+    if (n > INT32_MAX - 1 || width > INT32_MAX || num_free > INT32_MAX || max_tokens > INT32_MAX)
+        return set_error(RHZ_ERR_SHAPE, "n, width, num_free and max_tokens must fit int32");
+    RHZ_TRY(check_ptr(cu_seqlens, "cu_seqlens", 4, true));
+    RHZ_TRY(check_ptr(cursor_out, "cursor_out", 4, true));
+    RHZ_TRY(check_ptr(missing, "missing", 4, true));
+    RHZ_TRY(check_ptr(slot_map, "slot_map", 8, max_tokens > 0));
+    RHZ_TRY(check_ptr(block_table, "block_table", 4, n > 0 && width > 0));
+    RHZ_TRY(check_ptr(held_out, "held_out", 4, n > 0));
+    RHZ_TRY(check_ptr(cached, "cached", 4, n > 0));
+    RHZ_TRY(check_ptr(fresh, "fresh", 4, n > 0));
+    RHZ_TRY(check_ptr(held, "held", 4, n > 0));
+    RHZ_TRY(check_ptr(free_blocks, "free_blocks", 4, num_free > 0));
+    RHZ_TRY(check_ptr(cursor, "cursor", 4, cursor != nullptr));
+    // Every CTA reads held and cursor, so the results go elsewhere.
+    if (n > 0 && held_out == held) return set_error(RHZ_ERR_INVALID, "held_out must not be held itself");
+    if (cursor_out == cursor) return set_error(RHZ_ERR_INVALID, "cursor_out must not be cursor itself");
+    RHZ_TRY(require_sm100());
+    KvTablesArgs a{cu_seqlens, slot_map, block_table, held_out, cursor_out, missing, cached, fresh, held,
+                   free_blocks, cursor, n, width, num_free, max_tokens, page, as_cuda(stream)};
+    return launch_kv_tables(a);
+}
+
+int rhz_kv_append(void *k_cache, void *v_cache, const void *k, const void *v,
+                  const int64_t *slot_map, int64_t tokens, int64_t k_stride, int64_t v_stride,
+                  int64_t num_blocks, int32_t page, int32_t H_kv, int32_t d, int32_t dtype,
+                  rhz_stream_t stream) {
+    clear_error();
+    RHZ_TRY(check_dtype(dtype));
+    RHZ_TRY(check_heads(H_kv, d));
+    int shift = 0;
+    RHZ_TRY(check_page(page, &shift));
+    if (d % 4) return set_error(RHZ_ERR_SHAPE, "head_dim = %d: a multiple of 4", d);
+    if (tokens < 0 || num_blocks < 0)
+        return set_error(RHZ_ERR_SHAPE, "negative size (tokens %lld, num_blocks %lld)", (long long)tokens, (long long)num_blocks);
+    if (tokens > INT32_MAX || num_blocks > INT32_MAX)
+        return set_error(RHZ_ERR_SHAPE, "tokens and num_blocks must fit int32");
+    const int64_t row = static_cast<int64_t>(H_kv) * d;
+    if (k_stride < row || k_stride % 4 || v_stride < row || v_stride % 4)
+        return set_error(RHZ_ERR_SHAPE, "k_stride = %lld, v_stride = %lld: at least %lld and multiples of 4",
+                         (long long)k_stride, (long long)v_stride, (long long)row);
+    if (tokens == 0 || num_blocks == 0) return RHZ_OK;
+    const size_t unit = dtype == RHZ_DTYPE_BF16 ? 8 : 16;
+    RHZ_TRY(check_ptr(k_cache, "k_cache", 16, true));
+    RHZ_TRY(check_ptr(v_cache, "v_cache", 16, true));
+    RHZ_TRY(check_ptr(k, "k", unit, true));
+    RHZ_TRY(check_ptr(v, "v", unit, true));
+    RHZ_TRY(check_ptr(slot_map, "slot_map", 8, true));
+    RHZ_TRY(require_sm100());
+    KvAppendArgs a{k_cache, v_cache, k, v, slot_map, tokens, k_stride, v_stride, num_blocks, H_kv, d, page,
+                   dtype, as_cuda(stream)};
+    return launch_kv_append(a);
+}
+
+int rhz_attn_varlen_fwd(void *o, float *lse, const void *q, const void *k, const void *v,
+                        const int32_t *cu_seqlens, int64_t n_seq, int64_t total_tokens,
+                        int64_t q_stride, int64_t k_stride, int64_t v_stride, int32_t H,
+                        int32_t H_kv, int32_t d, float scale, int32_t dtype,
+                        rhz_stream_t stream) {
+    clear_error();
+    RHZ_TRY(check_attn_heads(H, H_kv, d, dtype));
+    RHZ_TRY(check_scale(scale));
+    RHZ_TRY(check_attn_sizes(n_seq, total_tokens, H));
+    RHZ_TRY(check_stride(q_stride, static_cast<int64_t>(H) * d, dtype, "q_stride"));
+    RHZ_TRY(check_stride(k_stride, static_cast<int64_t>(H_kv) * d, dtype, "k_stride"));
+    RHZ_TRY(check_stride(v_stride, static_cast<int64_t>(H_kv) * d, dtype, "v_stride"));
+    if (n_seq == 0 || total_tokens == 0) return RHZ_OK;
+    RHZ_TRY(check_ptr(o, "o", 16, true));
+    RHZ_TRY(check_ptr(q, "q", 16, true));
+    RHZ_TRY(check_ptr(k, "k", 16, true));
+    RHZ_TRY(check_ptr(v, "v", 16, true));
+    RHZ_TRY(check_ptr(cu_seqlens, "cu_seqlens", 4, true));
+    RHZ_TRY(check_ptr(lse, "lse", 4, lse != nullptr));
+    RHZ_TRY(require_sm100());
+    AttnArgs a{};
+    a.o = o; a.lse = lse; a.q = q; a.k = k; a.v = v;
+    a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+    a.cu_seqlens = cu_seqlens; a.n_seq = n_seq; a.total_tokens = total_tokens;
+    a.H = H; a.Hkv = H_kv; a.d = d; a.dtype = dtype; a.scale = scale;
+    a.most = total_tokens;
+    a.stream = as_cuda(stream);
+    return launch_attn(a);
+}
+
+int rhz_attn_tree_fwd(void *o, float *lse, const void *q, const void *k_cache,
+                      const void *v_cache, const int32_t *block_table, const int32_t *cached,
+                      const int32_t *cu_seqlens, const int32_t *parent, int64_t n_seq,
+                      int64_t total_tokens, int64_t max_positions, int64_t q_stride,
+                      int64_t width, int64_t num_blocks, int32_t page, int32_t H, int32_t H_kv,
+                      int32_t d, float scale, int32_t dtype, void *workspace,
+                      size_t workspace_bytes, rhz_stream_t stream) {
+    clear_error();
+    RHZ_TRY(check_attn_heads(H, H_kv, d, dtype));
+    RHZ_TRY(check_scale(scale));
+    RHZ_TRY(check_attn_sizes(n_seq, total_tokens, H));
+    int shift = 0;
+    RHZ_TRY(check_page(page, &shift));
+    if (max_positions < 0 || width < 0 || num_blocks < 0)
+        return set_error(RHZ_ERR_SHAPE, "negative size (max_positions %lld, width %lld, num_blocks %lld)",
+                         (long long)max_positions, (long long)width, (long long)num_blocks);
+    if (parent && max_positions > 64)
+        return set_error(RHZ_ERR_SHAPE, "a drafted tree has at most 64 positions (got %lld)", (long long)max_positions);
+    if (width << shift > INT32_MAX || num_blocks * H_kv > INT32_MAX >> shift)
+        return set_error(RHZ_ERR_SHAPE, "width * page = %lld positions or num_blocks * H_kv * page = %lld rows: beyond int32 indexing",
+                         (long long)(width << shift), (long long)((num_blocks * H_kv) << shift));
+    RHZ_TRY(check_stride(q_stride, static_cast<int64_t>(H) * d, dtype, "q_stride"));
+    if (n_seq == 0 || total_tokens == 0) return RHZ_OK;
+    RHZ_TRY(check_ptr(o, "o", 16, true));
+    RHZ_TRY(check_ptr(q, "q", 16, true));
+    RHZ_TRY(check_ptr(k_cache, "k_cache", 16, num_blocks > 0));
+    RHZ_TRY(check_ptr(v_cache, "v_cache", 16, num_blocks > 0));
+    RHZ_TRY(check_ptr(block_table, "block_table", 4, width > 0));
+    RHZ_TRY(check_ptr(cached, "cached", 4, true));
+    RHZ_TRY(check_ptr(cu_seqlens, "cu_seqlens", 4, true));
+    RHZ_TRY(check_ptr(parent, "parent", 4, parent != nullptr));
+    RHZ_TRY(check_ptr(lse, "lse", 4, lse != nullptr));
+    AttnArgs a{};
+    a.o = o; a.lse = lse; a.q = q; a.k = k_cache; a.v = v_cache;
+    a.q_stride = q_stride;
+    a.cu_seqlens = cu_seqlens; a.n_seq = n_seq; a.total_tokens = total_tokens;
+    a.H = H; a.Hkv = H_kv; a.d = d; a.dtype = dtype; a.scale = scale;
+    a.paged = true;
+    a.block_table = block_table; a.cached = cached; a.parent = parent;
+    a.width = width; a.num_blocks = num_blocks; a.shift = shift;
+    a.most = max_positions;
+    a.ws = workspace; a.ws_bytes = workspace_bytes;
+    a.stream = as_cuda(stream);
+    const size_t need = attn_ws_bytes(a);
+    if (need > 0) {
+        if (workspace == nullptr || workspace_bytes < need)
+            return set_error(RHZ_ERR_INVALID, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+        RHZ_TRY(check_ptr(workspace, "workspace", 256, true));
+    }
+    RHZ_TRY(require_sm100());
+    return launch_attn(a);
+}
+
+size_t rhz_attn_tree_workspace_bytes(int64_t total_tokens, int64_t max_positions, int64_t width,
+                                     int32_t page, int32_t H, int32_t H_kv, int32_t d,
+                                     int32_t dtype) {
+    clear_error();
+    int shift = 0;
+    if (check_attn_heads(H, H_kv, d, dtype) != RHZ_OK || check_page(page, &shift) != RHZ_OK ||
+        check_attn_sizes(0, total_tokens, H) != RHZ_OK || max_positions < 0 || width < 0 ||
+        width > INT32_MAX >> shift)
+        return 0;
+    AttnArgs a{};
+    a.total_tokens = total_tokens;
+    a.H = H; a.Hkv = H_kv; a.d = d; a.dtype = dtype;
+    a.paged = true;
+    a.width = width; a.shift = shift;
+    a.most = max_positions;
+    return attn_ws_bytes(a);
 }
 
 }  // extern "C"

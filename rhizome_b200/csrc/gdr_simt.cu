@@ -1,11 +1,13 @@
 // SIMT kernels of the GDR library (sm_100a):
 //   - gdr_step_kernel: one position of the recurrence for a ragged batch of
 //     sequences whose states live in a slot pool (decode, memory bound);
+//   - gdr_multistep_kernel, gdr_tree_kernel: a few drafted positions per
+//     sequence, a chain or a tree of them, with the state after every one;
 //   - gdr_seq_kernel: the recurrence applied position by position over whole
 //     sequences in fp32 (the rtol-1e-5 path, and the path for head widths the
 //     tensor-core kernel does not tile).
 //
-// Both follow gated_delta_step (crates/ops/src/delta.rs:93-127) per row:
+// All follow gated_delta_step (crates/ops/src/delta.rs:93-127) per row:
 //   sk_i = sum_j S_ij k_j
 //   S_ij <- alpha (S_ij - (beta sk_i) k_j) + (beta v_i) k_j
 //   o_i  = sum_j S_ij q_j
@@ -268,6 +270,123 @@ __global__ void __launch_bounds__(WARPS * 32)
     }
 }
 
+// ------------------------------------------------------------------ tree
+
+// The recurrence over a tree of drafted tokens: node t of sequence i starts
+// from the state of its parent node, S_t = step(S_parent(t)), or from the
+// pool's slot where the parent is -1, and every node's state is written out.
+// The rows of S never mix, so a warp that owns RPW rows walks the whole tree
+// by itself: a node whose parent is the node before it finds the parent's
+// rows in registers, any other reads back what this warp wrote for the parent
+// (the same lanes at the same addresses, so program order is enough). The
+// traffic that cannot be avoided is the d x d f32 state written per node and
+// head; k, q, v and the gates of the next node are loaded while the current
+// one is computed, so the serial chain is two row products and an update.
+template <typename T, int RPW, int NV, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32)
+    gdr_tree_kernel(T *__restrict__ o, float *states, const float *__restrict__ pool,
+                    const int32_t *__restrict__ slots, const int32_t *__restrict__ cu,
+                    const int32_t *__restrict__ parent, const T *__restrict__ q,
+                    const T *__restrict__ k, const T *__restrict__ v,
+                    const float *__restrict__ alpha, const float *__restrict__ beta,
+                    int64_t total, int most, int64_t num_slots, int H, int d, bool vec) {
+    const int64_t item = blockIdx.x;  // sequence * H + head
+    const int64_t seq = item / H;
+    const int h = static_cast<int>(item - seq * H);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row0 = blockIdx.y * (WARPS * RPW) + warp * RPW;
+    if (row0 >= d) return;
+    constexpr int SHIFT = 5 - Log2<RPW>::value;
+    const int myrow = row0 + (lane >> SHIFT);
+    const bool writer = (lane & ((1 << SHIFT) - 1)) == 0 && myrow < d;
+    const int64_t dd = static_cast<int64_t>(d) * d;
+    const int64_t first = min(max(static_cast<int64_t>(cu[seq]), int64_t{0}), total);
+    const int64_t last = min(max(static_cast<int64_t>(cu[seq + 1]), first), total);
+    const int m = static_cast<int>(min(last - first, static_cast<int64_t>(INT32_MAX)));
+    const int64_t slot = !pool ? 0 : slots ? static_cast<int64_t>(slots[seq]) : seq;
+    const bool valid = !pool || (slot >= 0 && slot < num_slots);
+    const float *root = pool && valid ? pool + (slot * H + h) * dd : nullptr;
+    const int64_t row_stride = static_cast<int64_t>(H) * d;
+
+    float s[RPW][NV][4];
+    auto fetch = [&](const float *S) {  // this warp's rows of a state, zeros without one
+#pragma unroll
+        for (int r = 0; r < RPW; ++r)
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+                const int j = 128 * c + 4 * lane;
+                if (S != nullptr && row0 + r < d) {
+                    load4(S + static_cast<int64_t>(row0 + r) * d + j, vec, nvalid(d, j), s[r][c]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[r][c][e] = 0.f;
+                }
+            }
+    };
+    float kk[NV][4], qq[NV][4], kn[NV][4], qn[NV][4], vn, an, bn;
+    int pn;
+    auto node = [&](int t) {  // the next node's inputs
+        const int64_t tok = first + t;
+        const int64_t at = tok * row_stride + static_cast<int64_t>(h) * d;
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int j = 128 * c + 4 * lane;
+            load4(k + at + j, vec, nvalid(d, j), kn[c]);
+            load4(q + at + j, vec, nvalid(d, j), qn[c]);
+        }
+        vn = myrow < d ? to_f32(v[at + myrow]) : 0.f;
+        an = alpha[tok * H + h];
+        bn = beta[tok * H + h];
+        pn = parent ? parent[tok] : t - 1;
+    };
+    uint64_t live = 0;  // nodes that take part: their parent is -1 or a live node before them
+    int held = -2;      // the node whose state the registers hold (-1: the root's)
+    const int nodes = min(m, most);
+    if (nodes > 0) node(0);
+    for (int t = 0; t < nodes; ++t) {
+        const int p = pn;
+        const float a = an, b = bn, vm = vn;
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                kk[c][e] = kn[c][e];
+                qq[c][e] = qn[c][e];
+            }
+        if (t + 1 < nodes) node(t + 1);
+        const int64_t tok = first + t;
+        T *op = o + tok * row_stride + static_cast<int64_t>(h) * d;
+        if (p < -1 || p >= t || (p >= 0 && !(live >> p & 1))) {
+            if (writer) op[myrow] = from_f32<T>(0.f);
+            continue;
+        }
+        live |= uint64_t{1} << t;
+        if (p != held) fetch(p < 0 ? root : states + ((first + p) * H + h) * dd);
+        held = t;
+        float vr[RPW], sk[RPW], ov[RPW], mine;
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) vr[r] = __shfl_sync(FULL, vm, r << SHIFT);
+        row_dots<RPW, NV>(s, kk, lane, sk, mine);
+        rank1_update<RPW, NV>(s, kk, sk, vr, a, b);
+        float *St = states + (tok * H + h) * dd;
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            if (row0 + r < d) {
+#pragma unroll
+                for (int c = 0; c < NV; ++c) {
+                    const int j = 128 * c + 4 * lane;
+                    store4(St + static_cast<int64_t>(row0 + r) * d + j, vec, nvalid(d, j), s[r][c]);
+                }
+            }
+        }
+        row_dots<RPW, NV>(s, qq, lane, ov, mine);
+        if (writer) op[myrow] = valid ? from_f32<T>(mine) : from_f32<T>(nanf(""));
+    }
+    for (int64_t t = nodes; t < m; ++t) {  // past the bound: not part of the tree
+        if (writer) o[(first + t) * row_stride + static_cast<int64_t>(h) * d + myrow] = from_f32<T>(0.f);
+    }
+}
+
 // ------------------------------------------------------------------ sequential
 
 // Tile of TS positions staged in shared memory: k and q rows (all d
@@ -474,7 +593,28 @@ int launch_multistep_t(const MultistepArgs &a) {
     return check_launch("gdr_multistep_kernel");
 }
 
+template <typename T, int RPW, int NV, int WARPS>
+int launch_tree_t(const TreeArgs &a) {
+    dim3 grid(static_cast<unsigned>(a.n * a.H), (a.d + WARPS * RPW - 1) / (WARPS * RPW));
+    const bool vec = (a.d % 4) == 0;
+    gdr_tree_kernel<T, RPW, NV, WARPS><<<grid, WARPS * 32, 0, a.stream>>>(
+        static_cast<T *>(a.o), a.states, a.pool, a.slots, a.cu_seqlens, a.parent,
+        static_cast<const T *>(a.q), static_cast<const T *>(a.k), static_cast<const T *>(a.v),
+        a.alpha, a.beta, a.total_tokens, a.most, a.num_slots, a.H, a.d, vec);
+    return check_launch("gdr_tree_kernel");
+}
+
 }  // namespace
+
+int launch_tree(const TreeArgs &a) {
+    if (a.n == 0 || a.total_tokens == 0) return RHZ_OK;
+    if (a.dtype == RHZ_DTYPE_BF16) {
+        if (a.d <= 128) return launch_tree_t<__nv_bfloat16, 8, 1, 8>(a);
+        return launch_tree_t<__nv_bfloat16, 4, 2, 8>(a);
+    }
+    if (a.d <= 128) return launch_tree_t<float, 8, 1, 8>(a);
+    return launch_tree_t<float, 4, 2, 8>(a);
+}
 
 int launch_multistep(const MultistepArgs &a) {
     if (a.n == 0 || a.Tn == 0) return RHZ_OK;

@@ -64,6 +64,71 @@ struct MultistepArgs {
     cudaStream_t stream;
 };
 
+// A tree of up to `most` (<= 64) drafted positions per packed sequence, the
+// state after each written out (gdr_simt.cu). parent == nullptr: a chain;
+// pool == nullptr: zero start.
+struct TreeArgs {
+    void *o;
+    float *states;
+    const float *pool;
+    const int32_t *slots, *cu_seqlens, *parent;
+    const void *q, *k, *v;
+    const float *alpha, *beta;
+    int64_t n, total_tokens;
+    int most;
+    int64_t num_slots;
+    int H, d, dtype;
+    cudaStream_t stream;
+};
+
+// Block tables and slot maps of one engine step (kv_cache.cu).
+struct KvTablesArgs {
+    int32_t *cu_seqlens;        // [n + 1]
+    int64_t *slot_map;          // [max_tokens]
+    int32_t *block_table;       // [n][width]
+    int32_t *held_out, *cursor_out, *missing;
+    const int32_t *cached, *fresh, *held, *free_blocks;
+    const int32_t *cursor;      // nullptr => 0
+    int64_t n, width, num_free, max_tokens;
+    int page;
+    cudaStream_t stream;
+};
+
+// K and V rows into the paged cache by slot (kv_cache.cu).
+struct KvAppendArgs {
+    void *k_cache, *v_cache;    // [num_blocks][H][page][d]
+    const void *k, *v;          // [tokens][H][d], tokens k_stride / v_stride elements apart
+    const int64_t *slot_map;    // [tokens]
+    int64_t tokens, k_stride, v_stride, num_blocks;
+    int H, d, page, dtype;
+    cudaStream_t stream;
+};
+
+// Softmax attention of the Global blocks with grouped heads (attn_simt.cu and
+// the tensor-core forms behind launch_attn). Sequence i owns query rows
+// [cu_seqlens[i], cu_seqlens[i+1]). Packed: its keys are the same rows of k
+// and v, causal. Paged: its keys are cached[i] cache positions and then its
+// own rows' positions, of which a row sees its ancestors in the drafted tree
+// (parent) or every earlier one (parent == nullptr).
+struct AttnArgs {
+    void *o;
+    float *lse;                 // [total_tokens][H] or nullptr
+    const void *q, *k, *v;      // paged: the caches [num_blocks][Hkv][page][d]
+    int64_t q_stride, k_stride, v_stride;  // elements between tokens (k, v: packed only)
+    const int32_t *cu_seqlens;
+    int64_t n_seq, total_tokens;
+    int H, Hkv, d, dtype;
+    float scale;
+    bool paged;
+    const int32_t *block_table, *cached, *parent;
+    int64_t width, num_blocks;
+    int shift;                  // log2 of the positions per page
+    int64_t most;               // rows of a sequence past this take no part
+    void *ws;                   // partial results of the split key axis (attn_ws_bytes)
+    size_t ws_bytes;
+    cudaStream_t stream;
+};
+
 // Input producer: conv + norms + gates in front of the recurrence (prep.cu).
 struct PrepArgs {
     void *q, *k, *v;
@@ -86,6 +151,14 @@ int launch_prep(const PrepArgs &a);
 // Sticky flag of the input producer's bounded TMA wait (1: a wait ran out).
 int prep_status(int *flag, bool clear);
 int launch_multistep(const MultistepArgs &a);
+int launch_tree(const TreeArgs &a);
+int launch_kv_tables(const KvTablesArgs &a);
+int launch_kv_append(const KvAppendArgs &a);
+int launch_attn(const AttnArgs &a);
+// Scratch of launch_attn (0: none); needs only the sizes of `a`.
+size_t attn_ws_bytes(const AttnArgs &a);
+// Sticky flag of the attention kernels' bounded waits (1: a wait ran out).
+int attn_status(int *flag, bool clear);
 int launch_seq(const SeqArgs &a);
 // Tensor-core chunked kernel (bf16, d == 128). Returns RHZ_ERR_SHAPE for
 // shapes it does not tile.

@@ -7,6 +7,7 @@ f32, states [n, H, d, d] f32 with S[i][j], i the v index and j the k index.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -109,6 +110,223 @@ def gdr_multistep(q, k, v, alpha, beta, max_positions=8, segment=None, state_poo
               _p(k), _p(v), _p(alpha), _p(beta), _p(segment), n, T, int(max_positions), num_slots,
               H, d, _dt(q), _stream(q.device))
     return outs, states
+
+
+def _on(dev: torch.device):
+    """The tensors' device as the current one for a launch on its stream."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _same_device(dev: torch.device, **tensors):
+    for name, x in tensors.items():
+        if x is not None and x.device != dev:
+            raise capi.InvalidArgument(capi.RHZ_ERR_INVALID, f"{name} is on {x.device}, not on {dev}")
+
+
+def _rows(x: torch.Tensor, name: str, dtype, tokens: int, H: int, d: int) -> int:
+    """Rows [tokens, H, d] whose tokens may lie apart (a slice of a fused
+    projection's output); returns the elements from one token to the next."""
+    if tuple(x.shape) != (tokens, H, d):
+        raise capi.ShapeError(capi.RHZ_ERR_SHAPE, f"{name} has shape {tuple(x.shape)}, expected {(tokens, H, d)}")
+    if x.dtype != dtype:
+        raise capi.DtypeError(capi.RHZ_ERR_DTYPE, f"{name} must be {dtype}, got {x.dtype}")
+    st = x.stride()
+    if (d > 1 and st[2] != 1) or (H > 1 and st[1] != d) or (tokens > 1 and st[0] < H * d):
+        raise capi.InvalidArgument(capi.RHZ_ERR_INVALID, f"{name}: each token's [H, d] must be contiguous (strides {st})")
+    if not x.is_cuda:
+        raise capi.InvalidArgument(capi.RHZ_ERR_INVALID, f"{name} must be a CUDA tensor")
+    return st[0] if tokens > 1 else H * d
+
+
+def _three(x: torch.Tensor, name: str):
+    if x.dim() != 3:
+        raise capi.ShapeError(capi.RHZ_ERR_SHAPE, f"{name} has shape {tuple(x.shape)}, expected [tokens, H, d]")
+    return x.shape
+
+
+def _index(x: torch.Tensor, name: str) -> int:
+    """A one-dimensional int32 array on the device; returns its length."""
+    if x.dim() != 1:
+        raise capi.ShapeError(capi.RHZ_ERR_SHAPE, f"{name} has shape {tuple(x.shape)}, expected one dimension")
+    _need(x, name, torch.int32)
+    return x.numel()
+
+
+def _cu(cu_seqlens: torch.Tensor) -> int:
+    n = _index(cu_seqlens, "cu_seqlens") - 1
+    if n < 0:
+        raise capi.ShapeError(capi.RHZ_ERR_SHAPE, "cu_seqlens needs at least one entry")
+    return n
+
+
+def gdr_tree_step(q, k, v, alpha, beta, cu_seqlens, parent, max_positions, state_pool=None,
+                  slot_idx=None, out=None, states=None):
+    """gdr_multistep over trees of drafted tokens: packed q/k/v [tokens, H, d],
+    sequence i's nodes are rows [cu_seqlens[i], cu_seqlens[i+1]) and parent
+    [tokens] int32 holds each node's parent within its sequence (-1: the
+    committed state in state_pool[slot_idx[i]]; None: a chain). Returns
+    (o [tokens, H, d], states [tokens, H, d, d]), the state after every node.
+    Nodes past the first max_positions (<= 64) of their sequence, and nodes
+    whose parent is neither -1 nor an earlier node that takes part, take no
+    part: o = 0 and their states are not written."""
+    tokens, _, _ = _three(q, "q")
+    H, d = _qkv(q, k, v, alpha, beta, (tokens,))
+    n = _cu(cu_seqlens)
+    if parent is not None:
+        _need(parent, "parent", torch.int32, (tokens,))
+    num_slots = 0 if state_pool is None else _pool(state_pool, "state_pool", H, d)
+    if slot_idx is not None:
+        _need(slot_idx, "slot_idx", torch.int32, (n,))
+    if out is not None:
+        _need(out, "out", q.dtype, tuple(q.shape))
+    if states is not None:
+        _need(states, "states", torch.float32, (tokens, H, d, d))
+    dev = q.device
+    _same_device(dev, k=k, v=v, alpha=alpha, beta=beta, cu_seqlens=cu_seqlens, parent=parent,
+                 state_pool=state_pool, slot_idx=slot_idx, out=out, states=states)
+    o = torch.empty_like(q) if out is None else out
+    if states is None:
+        states = torch.empty((tokens, H, d, d), device=dev, dtype=torch.float32)
+    with _on(dev):
+        capi.call("rhz_gdr_tree_step", _p(o), _p(states), _p(state_pool), _p(slot_idx),
+                  _p(cu_seqlens), _p(parent), _p(q), _p(k), _p(v), _p(alpha), _p(beta), n, tokens,
+                  int(max_positions), num_slots, H, d, _dt(q), _stream(dev))
+    return o, states
+
+
+# ---------------------------------------------------------------- Global blocks: paged cache and attention
+
+def kv_step_tables(cached, fresh, block_table, held, free_blocks, page, max_tokens, cursor=None):
+    """Block tables and slot maps of one engine step from request lengths, on
+    the device: request i has cached[i] positions in the cache, owns the first
+    held[i] entries of block_table[i] and adds fresh[i] positions; the pages
+    it lacks come from free_blocks[cursor:] in request order and are entered
+    into block_table in place. Returns (cu_seqlens [n + 1], slot_map
+    [max_tokens] int64, held [n], cursor [1], missing [1]): the packed rows'
+    offsets and cache slots (-1: no page, or past the last row), pages owned
+    and list position afterwards, and the pages that could not be had."""
+    n = _index(cached, "cached")
+    for name, x in (("fresh", fresh), ("held", held)):
+        _need(x, name, torch.int32, (n,))
+    if block_table.dim() != 2 or block_table.shape[0] != n:
+        raise capi.ShapeError(capi.RHZ_ERR_SHAPE, f"block_table has shape {tuple(block_table.shape)}, expected [{n}, width]")
+    _need(block_table, "block_table", torch.int32)
+    num_free = _index(free_blocks, "free_blocks")
+    if cursor is not None:
+        _need(cursor, "cursor", torch.int32, (1,))
+    if max_tokens < 0:
+        raise capi.ShapeError(capi.RHZ_ERR_SHAPE, f"max_tokens = {max_tokens}: must be >= 0")
+    dev = cached.device
+    _same_device(dev, fresh=fresh, held=held, block_table=block_table, free_blocks=free_blocks,
+                 cursor=cursor)
+    out = torch.empty(2 * n + 3, device=dev, dtype=torch.int32)
+    cu, held_out, cursor_out, missing = out.split((n + 1, n, 1, 1))
+    slot_map = torch.empty(max_tokens, device=dev, dtype=torch.int64)
+    with _on(dev):
+        capi.call("rhz_kv_step_tables", _p(cu), _p(slot_map), _p(block_table), _p(held_out),
+                  _p(cursor_out), _p(missing), _p(cached), _p(fresh), _p(held), _p(free_blocks),
+                  _p(cursor), n, block_table.shape[1], num_free, int(max_tokens), int(page),
+                  _stream(dev))
+    return cu, slot_map, held_out, cursor_out, missing
+
+
+def _caches(k_cache, v_cache, dtype):
+    """Caches [num_blocks, H_kv, page, d]; returns those sizes."""
+    if k_cache.dim() != 4:
+        raise capi.ShapeError(capi.RHZ_ERR_SHAPE, f"k_cache has shape {tuple(k_cache.shape)}, expected [num_blocks, H_kv, page, d]")
+    _need(k_cache, "k_cache", dtype)
+    _need(v_cache, "v_cache", dtype, tuple(k_cache.shape))
+    return k_cache.shape
+
+
+def kv_append(k, v, slot_map, k_cache, v_cache):
+    """K and V rows [tokens, H_kv, d] (slices of a fused projection will do)
+    into the caches [num_blocks, H_kv, page, d] at slot_map [tokens] int64
+    (block * page + row; rows with a slot outside the cache are skipped)."""
+    num_blocks, H, page, d = _caches(k_cache, v_cache, k.dtype)
+    tokens, _, _ = _three(k, "k")
+    ks, vs = _rows(k, "k", k.dtype, tokens, H, d), _rows(v, "v", k.dtype, tokens, H, d)
+    _need(slot_map, "slot_map", torch.int64, (tokens,))
+    dev = k.device
+    _same_device(dev, v=v, slot_map=slot_map, k_cache=k_cache, v_cache=v_cache)
+    with _on(dev):
+        capi.call("rhz_kv_append", _p(k_cache), _p(v_cache), _p(k), _p(v), _p(slot_map), tokens, ks,
+                  vs, num_blocks, page, H, d, _dt(k), _stream(dev))
+    return k_cache, v_cache
+
+
+def attn_varlen_fwd(q, k, v, cu_seqlens, scale=None, out=None, with_lse=False):
+    """Causal softmax attention over packed prompts, q [tokens, H, d], k and v
+    [tokens, H_kv, d] (slices of a fused projection will do): row t of a
+    sequence sees its sequence's rows up to itself; query head h reads K/V
+    head h // (H / H_kv). scale defaults to d ** -0.5. Returns o
+    [tokens, H, d], with_lse: (o, lse [tokens, H] f32)."""
+    tokens, H, d = _three(q, "q")
+    Hkv = _three(k, "k")[1]
+    qs = _rows(q, "q", q.dtype, tokens, H, d)
+    ks, vs = _rows(k, "k", q.dtype, tokens, Hkv, d), _rows(v, "v", q.dtype, tokens, Hkv, d)
+    n = _cu(cu_seqlens)
+    if out is not None:
+        _need(out, "out", q.dtype, (tokens, H, d))
+    dev = q.device
+    _same_device(dev, k=k, v=v, cu_seqlens=cu_seqlens, out=out)
+    o = torch.empty((tokens, H, d), device=dev, dtype=q.dtype) if out is None else out
+    lse = torch.empty((tokens, H), device=dev, dtype=torch.float32) if with_lse else None
+    with _on(dev):
+        capi.call("rhz_attn_varlen_fwd", _p(o), _p(lse), _p(q), _p(k), _p(v), _p(cu_seqlens), n,
+                  tokens, qs, ks, vs, H, Hkv, d, d ** -0.5 if scale is None else float(scale),
+                  _dt(q), _stream(dev))
+    return (o, lse) if with_lse else o
+
+
+def attn_tree_workspace_bytes(tokens: int, max_positions: int, width: int, page: int, H: int,
+                              H_kv: int, d: int, dtype: torch.dtype) -> int:
+    """Scratch of attn_tree_fwd for `tokens` query rows and tables of `width` pages."""
+    return int(capi.lib().rhz_attn_tree_workspace_bytes(tokens, max_positions, width, page, H, H_kv,
+                                                        d, _DTYPES.get(dtype, -1)))
+
+
+def attn_tree_fwd(q, k_cache, v_cache, block_table, cached, cu_seqlens, max_positions, parent=None,
+                  scale=None, out=None, with_lse=False, workspace=None):
+    """Softmax attention of drafted trees (or single tokens) over the paged
+    cache: q [tokens, H, d], sequence i's nodes are rows [cu_seqlens[i],
+    cu_seqlens[i+1]) and their own K and V are in the cache at positions
+    cached[i] + t (kv_append). A node sees the cached positions before, itself
+    and its ancestors by `parent` (as in gdr_tree_step; None: every node up to
+    itself). At most max_positions nodes of a sequence take part (64 with
+    `parent`); a node that takes no part gives o = 0, lse = -inf. Returns o,
+    with_lse: (o, lse [tokens, H] f32)."""
+    num_blocks, Hkv, page, d = _caches(k_cache, v_cache, q.dtype)
+    tokens, H, _ = _three(q, "q")
+    qs = _rows(q, "q", q.dtype, tokens, H, d)
+    n = _cu(cu_seqlens)
+    _need(cached, "cached", torch.int32, (n,))
+    if block_table.dim() != 2 or block_table.shape[0] != n:
+        raise capi.ShapeError(capi.RHZ_ERR_SHAPE, f"block_table has shape {tuple(block_table.shape)}, expected [{n}, width]")
+    _need(block_table, "block_table", torch.int32)
+    if parent is not None:
+        _need(parent, "parent", torch.int32, (tokens,))
+    if out is not None:
+        _need(out, "out", q.dtype, (tokens, H, d))
+    dev = q.device
+    _same_device(dev, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cached=cached,
+                 cu_seqlens=cu_seqlens, parent=parent, out=out)
+    width = block_table.shape[1]
+    o = torch.empty((tokens, H, d), device=dev, dtype=q.dtype) if out is None else out
+    lse = torch.empty((tokens, H), device=dev, dtype=torch.float32) if with_lse else None
+    ws, nbytes = None, 0
+    need = attn_tree_workspace_bytes(tokens, max_positions, width, page, H, Hkv, d, q.dtype)
+    if need > 0 or workspace is not None:
+        ws, nbytes = _workspace(workspace, need, dev)
+    with _on(dev):
+        capi.call("rhz_attn_tree_fwd", _p(o), _p(lse), _p(q), _p(k_cache), _p(v_cache),
+                  _p(block_table), _p(cached), _p(cu_seqlens), _p(parent), n, tokens,
+                  int(max_positions), qs, width, num_blocks, page, H, Hkv, d,
+                  d ** -0.5 if scale is None else float(scale), _dt(q), _p(ws), nbytes,
+                  _stream(dev))
+    return (o, lse) if with_lse else o
 
 
 def gdr_prep(xq, xk, xv, beta_logit, alpha_logit, a_head, conv_w, conv_b, conv_state=None,
