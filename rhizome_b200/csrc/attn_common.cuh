@@ -142,4 +142,10 @@ __device__ __forceinline__ Sight sight_of(const AttnArgs &a, const Seq &s, int64
 }
 
 }  // namespace attn
+
+// The tensor-core form (attn_tc.cu): bf16, d = 64 or 128.
+bool attn_tc_supports(const AttnArgs &a);
+int launch_attn_tc(const AttnArgs &a, const attn::Parts &parts, attn::Split split);
+int attn_tc_status(int *flag, bool clear);
+
 }  // namespace rhz

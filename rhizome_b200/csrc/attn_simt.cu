@@ -23,7 +23,7 @@ using namespace attn;
 
 constexpr int THREADS = 256;
 constexpr int KEYS = 64;                       // keys per tile
-constexpr Split SIMT_SPLIT{256, 64};
+constexpr Split SIMT_SPLIT{256, 64}, TC_SPLIT{2048, 64};
 
 // Four consecutive elements as f32 (d % 4 == 0, 16-byte aligned bases).
 __device__ __forceinline__ float4 get4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
@@ -347,23 +347,23 @@ int launch_join(const AttnArgs &a, const Parts &parts) {
 }
 
 template <typename T, int ROWS, int NG>
-int launch_simt_t(const AttnArgs &a, const Parts &parts, int64_t chunks) {
+int launch_simt_t(const AttnArgs &a, const Parts &parts, Split split) {
     const int smem = 4 * ((ROWS + KEYS) * (a.d + 4) + KEYS * a.d + ROWS * (KEYS + 4));
     const int tok = ROWS / (a.H / a.Hkv);
-    const int64_t units = (a.total_tokens / tok + a.n_seq) * chunks;
+    const int64_t units = (a.total_tokens / tok + a.n_seq) * parts.most;
     if (units > INT32_MAX) return set_error(RHZ_ERR_SHAPE, "attention over %lld units exceeds the grid", (long long)units);
     cudaError_t e = cudaFuncSetAttribute(attn_simt_kernel<T, ROWS, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return set_error(RHZ_ERR_DEVICE, "attn_simt_kernel: %s", cudaGetErrorString(e));
     dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(a.Hkv));
-    attn_simt_kernel<T, ROWS, NG><<<grid, THREADS, smem, a.stream>>>(a, parts, SIMT_SPLIT);
+    attn_simt_kernel<T, ROWS, NG><<<grid, THREADS, smem, a.stream>>>(a, parts, split);
     return check_launch("attn_simt_kernel");
 }
 
 template <typename T, int ROWS>
-int launch_simt_r(const AttnArgs &a, const Parts &parts, int64_t chunks) {
-    if (a.d <= 64) return launch_simt_t<T, ROWS, 1>(a, parts, chunks);
-    if (a.d <= 128) return launch_simt_t<T, ROWS, 2>(a, parts, chunks);
-    return launch_simt_t<T, ROWS, 4>(a, parts, chunks);
+int launch_simt_r(const AttnArgs &a, const Parts &parts, Split split) {
+    if (a.d <= 64) return launch_simt_t<T, ROWS, 1>(a, parts, split);
+    if (a.d <= 128) return launch_simt_t<T, ROWS, 2>(a, parts, split);
+    return launch_simt_t<T, ROWS, 4>(a, parts, split);
 }
 
 // The tokens a sequence may have at most: a paged call says so, a packed one
@@ -373,15 +373,17 @@ int64_t rows_bound(const AttnArgs &a) {
     return t * (a.H / a.Hkv);
 }
 
-int launch_simt(const AttnArgs &a, const Parts &parts, int64_t chunks) {
+int launch_simt(const AttnArgs &a, const Parts &parts, Split split) {
     const bool few = rows_bound(a) <= 16;  // (a group of more than 16 heads has more rows)
     if (a.dtype == RHZ_DTYPE_BF16)
-        return few ? launch_simt_r<__nv_bfloat16, 16>(a, parts, chunks) : launch_simt_r<__nv_bfloat16, 64>(a, parts, chunks);
-    return few ? launch_simt_r<float, 16>(a, parts, chunks) : launch_simt_r<float, 64>(a, parts, chunks);
+        return few ? launch_simt_r<__nv_bfloat16, 16>(a, parts, split) : launch_simt_r<__nv_bfloat16, 64>(a, parts, split);
+    return few ? launch_simt_r<float, 16>(a, parts, split) : launch_simt_r<float, 64>(a, parts, split);
 }
 
+Split split_of(const AttnArgs &a) { return attn_tc_supports(a) ? TC_SPLIT : SIMT_SPLIT; }
+
 int64_t chunk_bound(const AttnArgs &a) {
-    return a.paged ? SIMT_SPLIT.bound(a.width << a.shift) : 1;
+    return a.paged ? split_of(a).bound(a.width << a.shift) : 1;
 }
 
 }  // namespace
@@ -394,14 +396,14 @@ int launch_attn(const AttnArgs &a) {
     if (a.n_seq == 0 || a.total_tokens == 0) return RHZ_OK;
     const int64_t chunks = chunk_bound(a);
     const Parts parts = parts_at(a.ws, a.total_tokens, a.H, a.d, chunks);
-    const int st = launch_simt(a, parts, chunks);
+    const Split split = split_of(a);
+    // A cache of no pages has no tensor map; nothing is seen there.
+    const bool tc = attn_tc_supports(a) && !(a.paged && a.num_blocks == 0);
+    const int st = tc ? launch_attn_tc(a, parts, split) : launch_simt(a, parts, split);
     if (st != RHZ_OK || chunks <= 1) return st;
     return launch_join(a, parts);
 }
 
-int attn_status(int *flag, bool) {
-    *flag = 0;
-    return RHZ_OK;
-}
+int attn_status(int *flag, bool clear) { return attn_tc_status(flag, clear); }
 
 }  // namespace rhz
