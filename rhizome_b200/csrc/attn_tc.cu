@@ -25,6 +25,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "attn_common.cuh"
 #include "sm100.cuh"
@@ -41,6 +42,10 @@ constexpr int KEYS = 128;   // keys of a tile
 constexpr int THREADS = 384;  // the last warp only fills its warpgroup (registers move by warpgroup)
 constexpr int WARP_MMA = 8, WARP_TMA = 9, WARP_SCHED = 10;
 constexpr int GROUP = 256;  // sequences whose unit counts the scheduler holds at a time
+#ifndef POLY_
+#define POLY_ 0
+#endif
+constexpr int POLY = POLY_;      // of 8 pairs of exponentials, so many by polynomial
 constexpr float LAZY = 8.f; // a row's maximum may grow by 2^LAZY before O is rescaled
 
 // Sticky: a bounded wait of this kernel ran out.
@@ -60,10 +65,11 @@ template <int D>
 struct Cfg {
     static constexpr int HALVES = D / 64;
     static constexpr int TILE = KEYS * D * 2;              // a K, V or Q tile in bytes
-    static constexpr int STAGES = D == 128 ? 5 : 8;        // K and V tiles in flight
+    static constexpr int STAGES = D == 128 ? 4 : 8;        // K and V tiles in flight
     static constexpr int OFF_Q = 0;
     static constexpr int OFF_KV = 2 * TILE;
-    static constexpr int OFF_BAR = OFF_KV + STAGES * TILE; // barriers, units, scheduler's counts
+    static constexpr int OFF_OUT = OFF_KV + STAGES * TILE; // 4 KB per softmax warp: output rows on their way out
+    static constexpr int OFF_BAR = OFF_OUT + 8 * 4096;     // barriers, units, scheduler's counts
     static constexpr int OFF_UNIT = OFF_BAR + 256;
     static constexpr int OFF_MASK = OFF_UNIT + 128;
     static constexpr int OFF_MISC = OFF_MASK + 128;
@@ -76,7 +82,7 @@ struct Cfg {
 struct Bars {
     uint64_t kv_full[8], kv_empty[8];
     uint64_t q_full, q_empty;
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_full[2][2], o_full[2];  // P in two halves of 64 keys
     uint64_t u_full[2], u_empty[2];
     uint64_t drain;
 };
@@ -138,6 +144,29 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+// 2^x without the special-function unit, two at once: x = n + f with n the
+// nearest integer (the low bits of x + 1.5 * 2^23), |f| <= 1/2, then a
+// degree-5 polynomial in f (least maximal relative error among those with
+// constant term 1: 2^-22.4 in f32 arithmetic, as close as ex2.approx) and n
+// added to the exponent. x is held at -127, where f = 0 and the sum of
+// exponents is exactly 0.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    constexpr float MAGIC = 12582912.f;
+    x.x = fmaxf(x.x, -127.f);
+    x.y = fmaxf(x.y, -127.f);
+    const float2 t = add2(x, make_float2(MAGIC, MAGIC));
+    const float2 n = add2(t, make_float2(-MAGIC, -MAGIC));
+    const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 p = make_float2(0.001326472731307149f, 0.001326472731307149f);
+    p = fma2(p, f, make_float2(0.009671512991189957f, 0.009671512991189957f));
+    p = fma2(p, f, make_float2(0.05550733581185341f, 0.05550733581185341f));
+    p = fma2(p, f, make_float2(0.24022242426872253f, 0.24022242426872253f));
+    p = fma2(p, f, make_float2(0.6931470036506653f, 0.6931470036506653f));
+    p = fma2(p, f, make_float2(1.f, 1.f));
+    return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(p.x)),
+                       __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(p.y)));
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
@@ -156,7 +185,7 @@ __device__ __forceinline__ uint32_t seen_word(int all, uint64_t bits, int start)
 // that hold values which are not finite where some rows must not see them
 // (the tensor cores' 0 * NaN would reach every row of the tile).
 template <int D, bool PAGED>
-__device__ void plain_row(const TcArgs &g, const Unit &u, int row, const Sight &sight, int kend, int lane) {
+__device__ __noinline__ void plain_row(const TcArgs &g, const Unit &u, int row, const Sight &sight, int kend, int lane) {
     constexpr int C = D / 32;  // channels of a lane
     const AttnArgs &a = g.a;
     const int64_t token = u.first + u.t0 + row / g.group;
@@ -232,7 +261,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_init(&bar.q_empty, 1);
         for (int x = 0; x < 2; ++x) {
             mbar_init(&bar.s_full[x], 1);
-            mbar_init(&bar.p_full[x], 4);
+            mbar_init(&bar.p_full[x][0], 4);
+            mbar_init(&bar.p_full[x][1], 4);
             mbar_init(&bar.o_full[x], 1);
             mbar_init(&bar.u_full[x], 1);
             mbar_init(&bar.u_empty[x], 10);
@@ -313,8 +343,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         const uint32_t m = seen_word(all, sight.bits, key + 32 * w) & there[w];
+                        if (m != ~0u) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) v[w][e] = m >> e & 1u ? v[w][e] : -INFINITY;
+                            for (int e = 0; e < 32; ++e) v[w][e] = m >> e & 1u ? v[w][e] : -INFINITY;
+                        }
                     }
                     // V: rows behind the sequence or without a page become zero,
                     // values that are not finite in rows not everyone sees are noted.
@@ -322,11 +354,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const bool exists = key + r < u.keys && (!PAGED || (masks[vs][warp & 3] >> lane & 1u));
                     bool bad = false;
                     if (!exists || key + r >= full) {
-#pragma unroll
+#pragma unroll 1
                         for (int h = 0; h < C::HALVES; ++h)
-#pragma unroll
+#pragma unroll 2
                             for (int c = 0; c < 8; ++c) {
-                                uint4 *p = reinterpret_cast<uint4 *>(vrow + h * 16384 + c * 16);
+                                // (lanes start at different 16-byte pieces: different banks)
+                                uint4 *p = reinterpret_cast<uint4 *>(vrow + h * 16384 + ((c + lane) & 7) * 16);
                                 if (!exists) {
                                     *p = make_uint4(0u, 0u, 0u, 0u);
                                 } else {
@@ -367,23 +400,31 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const float from = top == -INFINITY ? 0.f : -top * g.c2;
                 const float2 c2 = make_float2(g.c2, g.c2), f2 = make_float2(from, from);
                 float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+auto exponentials = [&](auto poly) {  // pairs of each eight that go by polynomial
 #pragma unroll
-                for (int w = 0; w < 4; w += 2) {
-                    uint32_t p[32];
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t p[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        float2 y = fma2(make_float2(v[w + e / 16][2 * (e % 16)], v[w + e / 16][2 * (e % 16) + 1]), c2, f2);
-                        y.x = ex2(y.x);
-                        y.y = ex2(y.y);
-                        part[e & 1] = add2(part[e & 1], y);
-                        p[e] = pack_bf16(y.x, y.y);
+                        for (int e = 0; e < 32; ++e) {
+                            float2 y = fma2(make_float2(v[2 * half + e / 16][2 * (e % 16)], v[2 * half + e / 16][2 * (e % 16) + 1]), c2, f2);
+                            if (e % 8 < decltype(poly)::value) {
+                                y = ex2_poly(y);
+                            } else {
+                                y.x = ex2(y.x);
+                                y.y = ex2(y.y);
+                            }
+                            part[e & 1] = add2(part[e & 1], y);
+                            p[e] = pack_bf16(y.x, y.y);
+                        }
+                        tmem_st32u(ts + 32 * half, p);
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar.p_full[x][half]);
                     }
-                    tmem_st32u(ts + 16 * w, p);
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.p_full[x]);
+                };
+                if (edge) exponentials(std::integral_constant<int, 0>{});  // masked scores give exact zeros
+                else exponentials(std::integral_constant<int, POLY>{});
                 part[0] = add2(part[0], part[1]);
                 sum += part[0].x + part[0].y;
             }
@@ -409,34 +450,54 @@ __global__ void __launch_bounds__(THREADS, 1)
                         plain_row<D, PAGED>(g, u, x * g.tok * g.group + rr, theirs, kend, lane);
                 }
             } else {
+                // Rows leave through the warp's 4 KB of shared memory, 128 bytes of
+                // each at a time, so that eight lanes write a row's whole line (a
+                // thread writing its own row took 6,600 cycles per unit).
+                const bool split = PAGED && u.chunks > 1;
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
                 const float l2 = sum == 0.f ? -INFINITY : top * g.c2 + log2f(sum);
+                const uint32_t mine = used ? static_cast<uint32_t>(split ? g.parts.row(0, row, head) : row * a.H + head) : ~0u;
+                char *out = smem + C::OFF_OUT + warp * 4096;
+                char *dst = split ? reinterpret_cast<char *>(g.parts.o + g.parts.row(u.chunk, 0, 0) * D) : static_cast<char *>(a.o);
+                const int row_bytes = split ? D * 4 : D * 2;
+                auto leave = [&](int at) {  // 128 bytes of every row, from byte `at` of the row
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int rr = 4 * k + (lane >> 3);
+                        const uint32_t to = __shfl_sync(0xffffffffu, mine, rr);
+                        const uint4 q = *reinterpret_cast<const uint4 *>(out + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+                        if (to != ~0u) *reinterpret_cast<uint4 *>(dst + static_cast<int64_t>(to) * row_bytes + at + (lane & 7) * 16) = q;
+                    }
+                    __syncwarp();
+                };
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     float o[32];
-                    __syncwarp();
                     if (n > 0) {
                         tmem_ld32(to + c, o);
                         tmem_wait_ld();
                     }
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = n > 0 && !blind ? o[e] * inv : 0.f;
-                    if (!used) {
-                        // a row of the tile that has no token
-                    } else if (u.chunks > 1) {
-                        float4 *dst = reinterpret_cast<float4 *>(g.parts.o + g.parts.row(u.chunk, row, head) * D + c);
+                    if (split) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        for (int e = 0; e < 8; ++e)
+                            *reinterpret_cast<float4 *>(out + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                                make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        leave(c * 4);
                     } else {
-                        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.o) + (row * a.H + head) * D + c);
+                        const int h = (c & 32) >> 3;  // the row's lower or upper 64 bytes
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            dst[e] = make_uint4(pack_bf16(o[8 * e], o[8 * e + 1]), pack_bf16(o[8 * e + 2], o[8 * e + 3]),
-                                                pack_bf16(o[8 * e + 4], o[8 * e + 5]), pack_bf16(o[8 * e + 6], o[8 * e + 7]));
+                            *reinterpret_cast<uint4 *>(out + lane * 128 + (((h + e) ^ (lane & 7)) << 4)) =
+                                make_uint4(pack_bf16(o[8 * e], o[8 * e + 1]), pack_bf16(o[8 * e + 2], o[8 * e + 3]),
+                                           pack_bf16(o[8 * e + 4], o[8 * e + 5]), pack_bf16(o[8 * e + 6], o[8 * e + 7]));
+                        if (c & 32) leave((c - 32) * 2);
                     }
                 }
                 if (used) {
-                    if (u.chunks > 1) g.parts.lse[g.parts.row(u.chunk, row, head)] = l2;
+                    if (split) g.parts.lse[g.parts.row(u.chunk, row, head)] = l2;
                     else if (a.lse) a.lse[row * a.H + head] = l2 * LN2;
                 }
             }
@@ -450,95 +511,101 @@ __global__ void __launch_bounds__(THREADS, 1)
             // l / chunks (later blocks see more keys), and all sequences' units
             // of one l come together, the highest l first; dealt to the CTAs in
             // snake order.
-            const int pair = 2 * g.tok;
-            int64_t before = 0;      // units of the groups before this one
-            int64_t group = -1;
-            int64_t total = 0, level = 0, passed = 0;  // of this group: units, current l, units of higher l
-            int here = 0;            // sequences of the group with a unit l
+            // (The launch refuses more units than 31 bits count.)
+            const int pair = 2 * g.tok, n_seq = static_cast<int>(a.n_seq), G = gridDim.x;
+            int before = 0;                          // units of the groups before this one
+            int group = -1, total = 0, level = 0;    // of this group: units, current l
+            int passed = 0, here = 0;                // units of higher l, sequences with a unit l
             auto at_level = [&](int l) {
                 int n = 0;
+#pragma unroll 1
                 for (int i = lane; i < GROUP; i += 32) n += __popc(__ballot_sync(0xffffffffu, counts[i] > l));
                 return n;
             };
             bool going = true;
+#pragma unroll 1
             for (int i = 0; going; ++i) {
-                const int64_t G = gridDim.x;
-                const int64_t x = i * G + ((i & 1) ? G - 1 - blockIdx.x : blockIdx.x);
-                const int64_t want = x / a.Hkv;
+                const int64_t x64 = static_cast<int64_t>(i) * G + ((i & 1) ? G - 1 - blockIdx.x : blockIdx.x);
+                const int x = static_cast<int>(min(x64, static_cast<int64_t>(INT32_MAX)));
+                const int want = x / a.Hkv;
                 Unit u{};
-                while (true) {
-                    if (group >= 0 && want < before + total) break;
-                    before += group >= 0 ? total : 0;
+#pragma unroll 1
+                while (group < 0 || want - before >= total) {
+                    before += total;
                     ++group;
-                    if (group * GROUP >= a.n_seq) {
+                    if (group * GROUP >= n_seq) {
                         going = false;
                         break;
                     }
-                    int64_t sum = 0;
+                    total = 0;
                     int most = 0;
                     __syncwarp();
+#pragma unroll 1
                     for (int j = lane; j < GROUP; j += 32) {
-                        const int64_t q = group * GROUP + j;
-                        int64_t n = 0;
-                        if (q < a.n_seq) {
+                        const int q = group * GROUP + j;
+                        int n = 0;
+                        if (q < n_seq) {
                             const Seq s = seq_of(a, q);
-                            n = (s.m + pair - 1) / pair * (PAGED ? g.split.chunks(s.keys) : 1);
+                            n = (static_cast<int>(s.m) + pair - 1) / pair * (PAGED ? static_cast<int>(g.split.chunks(s.keys)) : 1);
                         }
-                        counts[j] = static_cast<int>(n);
-                        sum += n;
-                        most = max(most, static_cast<int>(n));
+                        counts[j] = n;
+                        total += n;
+                        most = max(most, n);
                     }
-                    for (int off = 16; off > 0; off >>= 1) {
-                        sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                        most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
-                    }
+                    total = __reduce_add_sync(0xffffffffu, total);
+                    most = __reduce_max_sync(0xffffffffu, most);
                     __syncwarp();
-                    total = sum;
                     level = most - 1;
                     passed = 0;
-                    here = most > 0 ? at_level(static_cast<int>(level)) : 0;
+                    here = most > 0 ? at_level(level) : 0;
                 }
                 if (going) {
+#pragma unroll 1
                     while (want - before >= passed + here) {
                         passed += here;
                         --level;
-                        here = at_level(static_cast<int>(level));
+                        here = at_level(level);
                     }
-                    int k = static_cast<int>(want - before - passed);  // the k-th sequence with a unit at this level
-                    int64_t q = 0;
+                    int k = want - before - passed;  // the k-th sequence with a unit at this level
+                    int q = 0;
+#pragma unroll 1
                     for (int j = 0; j < GROUP; j += 32) {
-                        const uint32_t b = __ballot_sync(0xffffffffu, counts[j + lane] > level);
-                        const int n = __popc(b);
-                        if (k < n) {
-                            q = group * GROUP + j + __fns(b, 0, k + 1);
+                        const bool has = counts[j + lane] > level;
+                        const uint32_t b = __ballot_sync(0xffffffffu, has);
+                        if (k < __popc(b)) {
+                            const uint32_t kth = __ballot_sync(0xffffffffu, has && __popc(b & ((1u << lane) - 1u)) == k);
+                            q = group * GROUP + j + __ffs(kth) - 1;
                             break;
                         }
-                        k -= n;
+                        k -= __popc(b);
                     }
                     const Seq s = seq_of(a, q);
-                    const int64_t chunks = PAGED ? g.split.chunks(s.keys) : 1;
+                    const int keys = static_cast<int>(s.keys), cached = static_cast<int>(s.cached);
+                    const int chunks = PAGED ? static_cast<int>(g.split.chunks(s.keys)) : 1;
                     u.valid = 1;
-                    u.seq = static_cast<int>(q);
-                    u.kvh = static_cast<int>(x % a.Hkv);
+                    u.seq = q;
+                    u.kvh = x - want * a.Hkv;
                     u.first = static_cast<int>(s.first);
                     u.m = static_cast<int>(s.m);
                     u.live = static_cast<int>(s.live);
-                    u.cached = static_cast<int>(s.cached);
-                    u.keys = static_cast<int>(s.keys);
-                    u.chunk = static_cast<int>(level % chunks);
-                    u.chunks = static_cast<int>(chunks);
-                    u.t0 = static_cast<int>(level / chunks) * pair;
-                    int64_t stop = s.keys;
+                    u.cached = cached;
+                    u.keys = keys;
+                    const int block = level / chunks;
+                    u.chunk = level - block * chunks;
+                    u.chunks = chunks;
+                    u.t0 = block * pair;
+                    int stop = keys;
                     if (PAGED) {
-                        const int64_t span = g.split.span(s.keys);
-                        u.kbeg = static_cast<int>(u.chunk * span);
+                        const int span = static_cast<int>(g.split.span(s.keys));
+                        u.kbeg = u.chunk * span;
                         stop = min(stop, u.kbeg + span);
                     }
+#pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        const int64_t t = u.t0 + static_cast<int64_t>(y) * g.tok;
-                        int64_t end = t >= s.live ? 0 : stop;
-                        if (!(PAGED && a.parent)) end = min(end, s.cached + t + g.tok);
-                        const int tiles = static_cast<int>(max((end - u.kbeg + KEYS - 1) / KEYS, int64_t{0}));
+                        const int t = u.t0 + y * g.tok;
+                        int end = t >= u.live ? 0 : stop;
+                        if (!(PAGED && a.parent)) end = min(end, cached + t + g.tok);
+                        const int tiles = max(end - u.kbeg + KEYS - 1, 0) / KEYS;
                         (y ? u.n1 : u.n0) = tiles;
                     }
                 }
@@ -633,25 +700,29 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int tiles = max(u.n0, u.n1);
                 if (tiles == 0) continue;
                 if (lane == 0) {
+                    // A descriptor's address field counts 16 bytes: steps are added to it.
+                    const uint64_t dq = sdesc_sw128(base + C::OFF_Q, 16, 1024);
+                    const uint64_t dk = sdesc_sw128(base + C::OFF_KV, 16, 1024);
+                    const uint64_t dv = sdesc_sw128(base + C::OFF_KV, 16384, 1024);
                     auto qk = [&](int x, int st) {
-                        const uint32_t qa = base + C::OFF_Q + x * C::TILE, ka = base + C::OFF_KV + st * C::TILE;
+                        const uint64_t qa = dq + x * (C::TILE >> 4), ka = dk + st * (C::TILE >> 4);
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k) {
-                            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-                            umma_f16(tmem + x * 128, sdesc_sw128(qa + off, 16, 1024), sdesc_sw128(ka + off, 16, 1024),
-                                     C::ID_QK, k > 0);
+                            const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                            umma_f16(tmem + x * 128, qa + off, ka + off, C::ID_QK, k > 0);
                         }
                         umma_commit(&bar.s_full[x]);
                     };
-                    auto pv = [&](int x, int st, bool more) {
-                        const uint32_t va = base + C::OFF_KV + st * C::TILE;
+                    auto pv = [&](int x, int st, int half, bool more) {
+                        const uint64_t va = dv + st * (C::TILE >> 4) + half * (8192 >> 4);
+                        const uint32_t p = tmem + x * 128 + half * 32;
 #pragma unroll
-                        for (int k = 0; k < KEYS / 16; ++k)
-                            umma_f16_ta(tmem + 256 + x * 128, tmem + x * 128 + 8 * k, sdesc_sw128(va + k * 2048, 16384, 1024),
-                                        C::ID_PV, more || k > 0);
+                        for (int k = 0; k < 4; ++k)
+                            umma_f16_ta(tmem + 256 + x * 128, p + 8 * k, va + k * (2048 >> 4), C::ID_PV, more || k + half > 0);
                     };
-                    ok = wait1(&bar.q_full, qn & 1, abort) && wait1(&bar.kv_full[it % C::STAGES], (it / C::STAGES) & 1, abort);
+                ok = wait1(&bar.q_full, qn & 1, abort) && wait1(&bar.kv_full[it % C::STAGES], (it / C::STAGES) & 1, abort);
                     if (ok) {
+#pragma unroll 1
                         for (int x = 0; x < 2; ++x)
                             if ((x ? u.n1 : u.n0) > 0) qk(x, it % C::STAGES);
                         umma_commit(&bar.kv_empty[it % C::STAGES]);
@@ -664,15 +735,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                         const int ks = kt % C::STAGES;
                         ok = wait1(&bar.kv_full[vs], (it / C::STAGES) & 1, abort);
                         bool have_k = false;
+#pragma unroll 1
                         for (int x = 0; ok && x < 2; ++x) {
                             const int n = x ? u.n1 : u.n0;
                             if (j < n) {
                                 uint32_t &pn = x ? pn1 : pn0;
-                                ok = wait1(&bar.p_full[x], pn & 1, abort);
+#pragma unroll 1
+                                for (int half = 0; ok && half < 2; ++half) {
+                                    ok = wait1(&bar.p_full[x][half], pn & 1, abort);
+                                    if (!ok) break;
+                                    tc_fence_after();
+                                    pv(x, vs, half, j > 0);
+                                }
                                 if (!ok) break;
                                 ++pn;
-                                tc_fence_after();
-                                pv(x, vs, j > 0);
                                 if (j + 1 == n) umma_commit(&bar.o_full[x]);
                             }
                             if (j + 1 < n) {
