@@ -39,8 +39,9 @@ using namespace sm100;
 
 constexpr int ROWS = 128;   // query rows of a tile
 constexpr int KEYS = 128;   // keys of a tile
-constexpr int THREADS = 384;  // the last warp only fills its warpgroup (registers move by warpgroup)
-constexpr int WARP_MMA = 8, WARP_TMA = 9, WARP_SCHED = 10;
+constexpr int HALF = 64;    // keys of a step
+constexpr int THREADS = 384;
+constexpr int WARP_MMA = 8, WARP_TMA = 10, WARP_SCHED = 11;  // (two of the first)
 constexpr int GROUP = 256;  // sequences whose unit counts the scheduler holds at a time
 #ifndef POLY_
 #define POLY_ 0
@@ -57,7 +58,7 @@ struct Unit {
     int32_t seq, kvh;
     int32_t first, t0, m, live;  // query rows: first row, this unit's first token, tokens, those taking part
     int32_t cached, keys;        // keys before the sequence's own, and in all
-    int32_t kbeg, n0, n1;        // first key, key tiles of either row tile
+    int32_t kbeg, n0, n1;        // first key, half key tiles of either row tile
     int32_t chunk, chunks;
 };
 
@@ -65,28 +66,29 @@ template <int D>
 struct Cfg {
     static constexpr int HALVES = D / 64;
     static constexpr int TILE = KEYS * D * 2;              // a K, V or Q tile in bytes
-    static constexpr int STAGES = D == 128 ? 4 : 8;        // K and V tiles in flight
+    static constexpr int STAGES = D == 128 ? 5 : 8;        // K and V tiles in flight
     static constexpr int OFF_Q = 0;
     static constexpr int OFF_KV = 2 * TILE;
-    static constexpr int OFF_OUT = OFF_KV + STAGES * TILE; // 4 KB per softmax warp: output rows on their way out
-    static constexpr int OFF_BAR = OFF_OUT + 8 * 4096;     // barriers, units, scheduler's counts
-    static constexpr int OFF_UNIT = OFF_BAR + 256;
-    static constexpr int OFF_MASK = OFF_UNIT + 128;
+    static constexpr int OFF_BAR = OFF_KV + STAGES * TILE; // barriers, units, scheduler's counts
+    static constexpr int OFF_UNIT = OFF_BAR + 320;
+    static constexpr int OFF_MASK = OFF_UNIT + 256;
     static constexpr int OFF_MISC = OFF_MASK + 128;
     static constexpr int OFF_COUNT = OFF_MISC + 64;
     static constexpr int BYTES = OFF_COUNT + GROUP * 4 + 1024;
-    static constexpr uint32_t ID_QK = idesc_bf16(ROWS, KEYS, false, false);
+    static constexpr uint32_t ID_QK = idesc_bf16(ROWS, HALF, false, false);
     static constexpr uint32_t ID_PV = idesc_bf16(ROWS, D, false, true);
 };
 
-struct Bars {
-    uint64_t kv_full[8], kv_empty[8];
-    uint64_t q_full, q_empty;
-    uint64_t s_full[2], p_full[2][2], o_full[2];  // P in two halves of 64 keys
-    uint64_t u_full[2], u_empty[2];
-    uint64_t drain;
+// Barriers, 8 bytes each, from OFF_BAR. Everything in shared memory that the
+// main loop touches is addressed by 32-bit addresses: as generic pointers the
+// loop's invariants alone would push its score registers out to memory.
+enum Bar : uint32_t {
+    KV_FULL = 0, KV_EMPTY = 8, Q_FULL = 16, Q_EMPTY = 17,
+    S_FULL = 18, P_FULL = 22,  // [row tile][half of the key tile]
+    PV_DONE = 26, O_FULL = 28, // [row tile]: a step's output product, a unit's last
+    U_FULL = 30, U_EMPTY = 34, DRAIN = 38, NUM_BARS = 39
 };
-static_assert(sizeof(Bars) <= 256 && 2 * sizeof(Unit) <= 128, "shared-memory layout");
+static_assert(NUM_BARS * 8 <= 320 && 4 * sizeof(Unit) <= 256, "shared-memory layout");
 
 struct TcArgs {
     AttnArgs a;
@@ -98,26 +100,104 @@ struct TcArgs {
     float c2;    // scale * log2 e
 };
 
-// Bounded wait of one thread that also ends when another role gave up.
-__device__ bool wait1(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63u) == 0) {
-            if (*abort) return false;
-            if (globaltimer_ns() - t0 > 2000000000ull) {
-                *abort = 1;
-                atomicExch(&g_attn_timeout, 1);
-                return false;
-            }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"  // suspended for about 1 us at most
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
+// D[tmem] (+)= A * B, bf16 with f32 sums: descriptors as their low words and
+// the high word that they share; A in shared memory, or in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool more) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(more))
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool more) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(more))
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t lds(uint32_t at) {
+    uint32_t x;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+    return x;
+}
+__device__ __forceinline__ void sts(uint32_t at, uint32_t x) {
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(x) : "memory");
+}
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap *tm, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap *tm, int c0, int c1, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+
+// Bounded wait of one thread (2^21 tries, some 0.1 to 2 s) that also ends when
+// another role gave up; *stop in shared memory tells the others.
+__device__ __forceinline__ bool wait1(uint32_t bar, uint32_t parity, uint32_t stop) {
+    for (uint32_t i = 0; !bar_try(bar, parity); ++i) {
+        if ((i & 63u) != 63u) continue;
+        if (lds(stop) != 0) return false;
+        if (i >= (1u << 21)) {
+            sts(stop, 1);
+            atomicExch(&g_attn_timeout, 1);
+            return false;
         }
+    }
+    return true;
+}
+
+// For copies and products in flight when a role gave up: bounded the same way.
+__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < (1u << 20) && !bar_try(bar, parity); ++i) {
     }
 }
 
 // The same for a whole warp: all its lanes go on or none does.
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    return __all_sync(0xffffffffu, wait1(bar, parity, abort));
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t stop) {
+    return __all_sync(0xffffffffu, wait1(bar, parity, stop));
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -167,10 +247,42 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
                        __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(p.y)));
 }
 
+// 8 consecutive 32-bit columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
+
+// 32 bytes of a row: one store where the address allows it.
+__device__ __forceinline__ void store32(void *p, const uint32_t (&w)[8], bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                     "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    } else {
+        static_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        static_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+
+__device__ __forceinline__ bool aligned32(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 
 // Bits of the 32 keys from `start` that a row sees (`all`: keys below it are
 // seen; `bits`: the 64 keys from `all` on).
@@ -239,37 +351,39 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ char smem_raw[];
     char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
     const uint32_t base = smem_u32(smem);
-    Bars &bar = *reinterpret_cast<Bars *>(smem + C::OFF_BAR);
+    const uint32_t bars = base + C::OFF_BAR, abort = base + C::OFF_MISC + 4;
     Unit *units = reinterpret_cast<Unit *>(smem + C::OFF_UNIT);
-    uint32_t(*masks)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + C::OFF_MASK);  // per ring stage: keys with memory behind them
+    const uint32_t masks = base + C::OFF_MASK;  // 16 bytes per ring stage: keys with memory behind them
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
-    volatile int *abort = reinterpret_cast<volatile int *>(smem + C::OFF_MISC + 4);
     // Unit i of tile x met values that are not finite where not every row sees
-    // them: [x][i & 3] == i + 1. (A warp that sets the flag of unit i + 4 has
-    // seen the descriptor of i + 4, so every warp has read that of i + 2 and is done with i.)
-    volatile int(*spoiled)[4] = reinterpret_cast<volatile int(*)[4]>(smem + C::OFF_MISC + 16);
+    // them: word [x][i & 3] is i + 1. (Unit i + 4 comes when every warp is done with i.)
+    const uint32_t spoiled = base + C::OFF_MISC + 16;
     int *counts = reinterpret_cast<int *>(smem + C::OFF_COUNT);
     const AttnArgs &a = g.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; ++i) {
-            mbar_init(&bar.kv_full[i], 1);
-            mbar_init(&bar.kv_empty[i], 1);
+            bar_init(bars + 8 * (KV_FULL + i), 1);
+            bar_init(bars + 8 * (KV_EMPTY + i), 2);
         }
-        mbar_init(&bar.q_full, 1);
-        mbar_init(&bar.q_empty, 1);
+        bar_init(bars + 8 * Q_FULL, 1);
+        bar_init(bars + 8 * Q_EMPTY, 2);
         for (int x = 0; x < 2; ++x) {
-            mbar_init(&bar.s_full[x], 1);
-            mbar_init(&bar.p_full[x][0], 4);
-            mbar_init(&bar.p_full[x][1], 4);
-            mbar_init(&bar.o_full[x], 1);
-            mbar_init(&bar.u_full[x], 1);
-            mbar_init(&bar.u_empty[x], 10);
+            bar_init(bars + 8 * (PV_DONE + x), 1);
+            bar_init(bars + 8 * (O_FULL + x), 1);
+            for (int h = 0; h < 2; ++h) {
+                bar_init(bars + 8 * (S_FULL + 2 * x + h), 1);
+                bar_init(bars + 8 * (P_FULL + 2 * x + h), 4);
+            }
         }
-        mbar_init(&bar.drain, 1);
-        *abort = 0;
-        for (int i = 0; i < 8; ++i) spoiled[i >> 2][i & 3] = 0;
+        for (int i = 0; i < 4; ++i) {
+            bar_init(bars + 8 * (U_FULL + i), 1);
+            bar_init(bars + 8 * (U_EMPTY + i), WARP_SCHED);
+        }
+        bar_init(bars + 8 * DRAIN, 2);
+        sts(abort, 0);
+        for (int i = 0; i < 8; ++i) sts(spoiled + 4 * i, 0);
         mbar_fence_init();
     }
     if (warp == WARP_MMA) tmem_alloc(tmem_slot, 512);
@@ -283,226 +397,249 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // Units come through a ring of two.
+    // Units come through a ring of four. The copying and the issuing warp take
+    // theirs out at once, the softmax warps leave it there until they are done.
     auto next_unit = [&](int i, Unit &u) -> bool {
-        if (!wait(&bar.u_full[i & 1], (i >> 1) & 1, abort)) return false;
-        u = units[i & 1];
+        if (!wait(bars + 8 * (U_FULL + (i & 3)), (i >> 2) & 1, abort)) return false;
+        u = units[i & 3];
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.u_empty[i & 1]);
+        if (lane == 0) bar_arrive(bars + 8 * (U_EMPTY + (i & 3)));
         return u.valid != 0;
     };
 
     // 384 x 168 registers at launch: 256 x 208 for the softmax, 128 x 88 for the rest.
-    if (warp < 8) {
+    if (warp < WARP_MMA) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // Softmax of tile x: thread r of the warpgroup is row r.
         const int x = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + 256 + x * 128;
-        Unit u;
-        uint32_t sn = 0, on = 0, it = 0;  // S tiles and outputs waited for, ring position of the unit's first tile
-        for (int i = 0; next_unit(i, u); ++i) {
-            const int token = u.t0 + x * g.tok + r / g.group;
-            const bool used = r < g.tok * g.group && token < u.m;
-            Seq s;
-            s.first = u.first; s.m = u.m; s.live = u.live; s.cached = u.cached; s.keys = u.keys;
-            Sight sight{0, 0};
-            if (used) sight = sight_of(a, s, token);
-            const int all = static_cast<int>(sight.all);
+        uint32_t sn = 0, on = 0, it = 0;  // steps and units done (mod 2^32) of this row tile, ring position of the unit's first tile
+        uint32_t sp = 0;          // phases of S_FULL waited for, one bit per half
+        for (int i = 0; wait(bars + 8 * (U_FULL + (i & 3)), (i >> 2) & 1, abort); ++i) {
+            const Unit &u = units[i & 3];
+            if (!u.valid) break;
+            int all = 0;         // what the row sees: keys below `all`, and of the 64 from there on those in `bits`
+            uint64_t bits = 0;
+            {
+                const int token = u.t0 + x * g.tok + r / g.group;
+                if (r < g.tok * g.group && token < u.m) {
+                    Seq s;
+                    s.first = u.first; s.m = u.m; s.live = u.live; s.cached = u.cached; s.keys = u.keys;
+                    const Sight sight = sight_of(a, s, token);
+                    all = static_cast<int>(sight.all);
+                    if (PAGED) bits = sight.bits;
+                }
+            }
             // Tiles below `full` are seen whole by every live row of the warpgroup's tile.
-            const int t_first = u.t0 + x * g.tok;
-            const int full = PAGED && a.parent ? u.cached : u.cached + t_first + 1;
+            const int full = PAGED && a.parent ? u.cached : u.cached + u.t0 + x * g.tok + 1;
+            const int kbeg = u.kbeg;
             float top = -INFINITY, sum = 0.f;
             bool ok = true;
             const int n = x ? u.n1 : u.n0;
-            for (int j = 0; j < n; ++j, ++sn) {
-                const int key = u.kbeg + j * KEYS;
-                bool edge = key + KEYS > full;
-                const uint32_t vt = it + 2 * j + 1;  // this tile's V in the ring
-                const int vs = vt % C::STAGES;
-                uint32_t there[4] = {~0u, ~0u, ~0u, ~0u};
+            for (int e = 0; e < n; ++e, ++sn) {
+                const int h = e & 1, key = kbeg + e * HALF;
+                bool edge = key + HALF > full;
+                uint32_t there[2] = {~0u, ~0u};
                 if (PAGED || edge) {
-                    ok = wait(&bar.kv_full[vs], (vt / C::STAGES) & 1, abort);
+                    const uint32_t vt = it + (e | 1);  // this tile's V in the ring
+                    const int vs = vt % C::STAGES;
+                    ok = wait(bars + 8 * (KV_FULL + vs), (vt / C::STAGES) & 1, abort);
                     if (!ok) break;
                     if (PAGED) {
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            there[w] = masks[vs][w];
+                        for (int w = 0; w < 2; ++w) {
+                            there[w] = lds(masks + 16 * vs + 8 * h + 4 * w);
                             edge |= there[w] != ~0u;
                         }
                     }
-                }
-                ok = wait(&bar.s_full[x], sn & 1, abort);
-                if (!ok) break;
-                tc_fence_after();
-                float v[4][32];
+                    if (edge) {
+                        // V: rows behind the sequence or without a page become zero,
+                        // values that are not finite in rows not everyone sees are
+                        // noted. Two threads to a key's row.
+                        const int kr = r >> 1;
+                        const uint32_t vrow = base + C::OFF_KV + vs * C::TILE + (h * HALF + kr) * 128 + (D == 128 ? (r & 1) * 16384 : 0);
+                        const bool exists = key + kr < u.keys && (!PAGED || (lds(masks + 16 * vs + 8 * h + 4 * (kr >> 5)) >> (kr & 31) & 1u));
+                        if (!exists || key + kr >= full) {
+                            bool bad = false;
+#pragma unroll 2
+                            for (int c = 0; c < D / 16; ++c) {  // 16-byte pieces; lanes start at different ones: different banks
+                                const int piece = D == 128 ? ((c + (lane >> 1)) & 7) : ((c + (lane >> 1)) & 3) + 4 * (r & 1);
+                                const uint32_t at = vrow + piece * 16;
+                                if (!exists) {
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                                } else {
+                                    uint32_t ws[4];
+                                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                                 : "=r"(ws[0]), "=r"(ws[1]), "=r"(ws[2]), "=r"(ws[3])
+                                                 : "r"(at)
+                                                 : "memory");
 #pragma unroll
-                for (int w = 0; w < 4; ++w) tmem_ld32(ts + 32 * w, v[w]);
+                                    for (int k = 0; k < 4; ++k)
+                                        bad |= (ws[k] & 0x7f80u) == 0x7f80u || (ws[k] & 0x7f800000u) == 0x7f800000u;
+                                }
+                            }
+                            if (bad) sts(spoiled + 16 * x + 4 * (i & 3), i + 1);
+                        }
+                        fence_proxy_async_smem();
+                    }
+                }
+                ok = wait(bars + 8 * (S_FULL + 2 * x + h), sp >> h & 1, abort);
+                if (!ok) break;
+                sp ^= 1u << h;
+                tc_fence_after();
+                float v[2][32];
+#pragma unroll
+                for (int w = 0; w < 2; ++w) tmem_ld32(ts + HALF * h + 32 * w, v[w]);
                 tmem_wait_ld();
                 if (edge) {
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t m = seen_word(all, sight.bits, key + 32 * w) & there[w];
+                    for (int w = 0; w < 2; ++w) {
+                        const uint32_t m = seen_word(all, bits, key + 32 * w) & there[w];
                         if (m != ~0u) {
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) v[w][e] = m >> e & 1u ? v[w][e] : -INFINITY;
+                            for (int k = 0; k < 32; ++k) v[w][k] = m >> k & 1u ? v[w][k] : -INFINITY;
                         }
                     }
-                    // V: rows behind the sequence or without a page become zero,
-                    // values that are not finite in rows not everyone sees are noted.
-                    char *vrow = smem + C::OFF_KV + vs * C::TILE + r * 128;
-                    const bool exists = key + r < u.keys && (!PAGED || (masks[vs][warp & 3] >> lane & 1u));
-                    bool bad = false;
-                    if (!exists || key + r >= full) {
-#pragma unroll 1
-                        for (int h = 0; h < C::HALVES; ++h)
-#pragma unroll 2
-                            for (int c = 0; c < 8; ++c) {
-                                // (lanes start at different 16-byte pieces: different banks)
-                                uint4 *p = reinterpret_cast<uint4 *>(vrow + h * 16384 + ((c + lane) & 7) * 16);
-                                if (!exists) {
-                                    *p = make_uint4(0u, 0u, 0u, 0u);
-                                } else {
-                                    const uint4 q = *p;
-                                    const uint32_t ws[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e)
-                                        bad |= (ws[e] & 0x7f80u) == 0x7f80u || (ws[e] & 0x7f800000u) == 0x7f800000u;
-                                }
-                            }
-                    }
-                    if (bad) spoiled[x][i & 3] = i + 1;
-                    fence_proxy_async_smem();
                 }
                 float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
+                for (int k = 0; k < 32; k += 4)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) best[w] = fmaxf(best[w], v[w][e]);
-                const float peak = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-                if (j == 0) {
+                    for (int w = 0; w < 4; ++w) best[w] = max3(best[w], v[w >> 1][k + 2 * (w & 1)], v[w >> 1][k + 2 * (w & 1) + 1]);
+                const float peak = fmaxf(max3(best[0], best[1], best[2]), best[3]);
+                if (e == 0) {
                     top = peak;
                 } else if (__any_sync(0xffffffffu, (peak - top) * g.c2 > LAZY)) {
                     const float now = fmaxf(top, peak);
                     const float keep = now == top ? 1.f : ex2((top - now) * g.c2);
                     top = now;
                     sum *= keep;
+                    // O holds every step before this one (that step sn - 2 is done follows
+                    // from S, so the parity tells step sn - 1 from it)
+                    ok = wait(bars + 8 * (PV_DONE + x), (sn - 1) & 1, abort);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        tmem_ld32(to + c, o);
+                    for (int c = 0; c < D; c += 8) {  // few registers: the scores are held meanwhile
+                        uint32_t o[8];
+                        tmem_ld8(to + c, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= keep;
-                        tmem_st32(to + c, o);
+                        for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                        tmem_st8(to + c, o);
                     }
                 }
                 const float from = top == -INFINITY ? 0.f : -top * g.c2;
                 const float2 c2 = make_float2(g.c2, g.c2), f2 = make_float2(from, from);
                 float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-auto exponentials = [&](auto poly) {  // pairs of each eight that go by polynomial
+                auto exponentials = [&](auto poly) {  // pairs of each eight that go by polynomial
+                    uint32_t p[32];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t p[32];
+                    for (int b = 0; b < 32; b += 8) {
+                        float2 y[8];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            float2 y = fma2(make_float2(v[2 * half + e / 16][2 * (e % 16)], v[2 * half + e / 16][2 * (e % 16) + 1]), c2, f2);
-                            if (e % 8 < decltype(poly)::value) {
-                                y = ex2_poly(y);
-                            } else {
-                                y.x = ex2(y.x);
-                                y.y = ex2(y.y);
-                            }
-                            part[e & 1] = add2(part[e & 1], y);
-                            p[e] = pack_bf16(y.x, y.y);
+                        for (int k = 0; k < 8; ++k) {
+                            const int c = 2 * (b + k);
+                            y[k] = fma2(make_float2(v[c / 32][c % 32], v[c / 32][c % 32 + 1]), c2, f2);
                         }
-                        tmem_st32u(ts + 32 * half, p);
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&bar.p_full[x][half]);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            if (k < decltype(poly)::value) {
+                                y[k] = ex2_poly(y[k]);
+                            } else {
+                                y[k].x = ex2(y[k].x);
+                                y[k].y = ex2(y[k].y);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            part[k & 1] = add2(part[k & 1], y[k]);
+                            p[b + k] = pack_bf16(y[k].x, y[k].y);
+                        }
                     }
+                    tmem_st32u(ts + HALF * h, p);
                 };
-                if (edge) exponentials(std::integral_constant<int, 0>{});  // masked scores give exact zeros
+                if (POLY == 0 || edge) exponentials(std::integral_constant<int, 0>{});  // masked scores give exact zeros
                 else exponentials(std::integral_constant<int, POLY>{});
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(bars + 8 * (P_FULL + 2 * x + h));
                 part[0] = add2(part[0], part[1]);
                 sum += part[0].x + part[0].y;
             }
             if (!ok) break;
-            it += 2 * max(u.n0, u.n1);
+            it += 2 * ((max(u.n0, u.n1) + 1) / 2);
             bool bad = false;
             if (n > 0) {
-                if (!wait(&bar.o_full[x], on & 1, abort)) break;
+                if (!wait(bars + 8 * (O_FULL + x), on & 1, abort)) break;
                 ++on;
                 tc_fence_after();
-                bad = spoiled[x][i & 3] == i + 1;  // written before its warp's last p_full arrival
+                bad = lds(spoiled + 16 * x + 4 * (i & 3)) == i + 1;  // written before its warp's last p_full arrival
             }
-            const bool blind = sight.all == 0 && sight.bits == 0;  // sees nothing: whole tiles above did not ask
+            const bool blind = all == 0 && bits == 0;  // sees nothing: whole tiles above did not ask
             if (blind) sum = 0.f;
+            const int token = u.t0 + x * g.tok + r / g.group;
+            const bool used = r < g.tok * g.group && token < u.m;
             const int64_t row = u.first + token;
             const int head = u.kvh * g.group + r % g.group;
+            const bool split = PAGED && u.chunks > 1;
             if (bad) {
-                const int kend = min(u.keys, u.kbeg + n * KEYS);
+                const int kend = min(u.keys, u.kbeg + n * HALF);
                 for (int w = 0; w < 32; ++w) {  // the warp takes its own 32 rows
                     const int rr = (warp & 3) * 32 + w;
-                    const Sight theirs{__shfl_sync(0xffffffffu, sight.all, w), __shfl_sync(0xffffffffu, sight.bits, w)};
+                    const Sight theirs{__shfl_sync(0xffffffffu, all, w), __shfl_sync(0xffffffffu, bits, w)};
                     if (__shfl_sync(0xffffffffu, static_cast<int>(used), w))
                         plain_row<D, PAGED>(g, u, x * g.tok * g.group + rr, theirs, kend, lane);
                 }
             } else {
-                // Rows leave through the warp's 4 KB of shared memory, 128 bytes of
-                // each at a time, so that eight lanes write a row's whole line (a
-                // thread writing its own row took 6,600 cycles per unit).
-                const bool split = PAGED && u.chunks > 1;
+                // A thread writes its row's 32 bytes at a time: whole sectors.
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const float l2 = sum == 0.f ? -INFINITY : top * g.c2 + log2f(sum);
-                const uint32_t mine = used ? static_cast<uint32_t>(split ? g.parts.row(0, row, head) : row * a.H + head) : ~0u;
-                char *out = smem + C::OFF_OUT + warp * 4096;
-                char *dst = split ? reinterpret_cast<char *>(g.parts.o + g.parts.row(u.chunk, 0, 0) * D) : static_cast<char *>(a.o);
-                const int row_bytes = split ? D * 4 : D * 2;
-                auto leave = [&](int at) {  // 128 bytes of every row, from byte `at` of the row
-                    __syncwarp();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int rr = 4 * k + (lane >> 3);
-                        const uint32_t to = __shfl_sync(0xffffffffu, mine, rr);
-                        const uint4 q = *reinterpret_cast<const uint4 *>(out + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-                        if (to != ~0u) *reinterpret_cast<uint4 *>(dst + static_cast<int64_t>(to) * row_bytes + at + (lane & 7) * 16) = q;
-                    }
-                    __syncwarp();
-                };
+                float *po = g.parts.o + g.parts.row(u.chunk, row, head) * D;
+                __nv_bfloat16 *bo = static_cast<__nv_bfloat16 *>(a.o) + (row * a.H + head) * D;
+                const bool wide = aligned32(a.o);
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     float o[32];
+                    __syncwarp();
                     if (n > 0) {
                         tmem_ld32(to + c, o);
                         tmem_wait_ld();
                     }
+                    if (n == 0 || blind) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = n > 0 && !blind ? o[e] * inv : 0.f;
-                    if (split) {
+                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                    }
+                    if (used && split) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            *reinterpret_cast<float4 *>(out + lane * 128 + ((e ^ (lane & 7)) << 4)) =
-                                make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                        leave(c * 4);
-                    } else {
-                        const int h = (c & 32) >> 3;  // the row's lower or upper 64 bytes
+                        for (int e = 0; e < 32; e += 8) {
+                            uint32_t w[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            *reinterpret_cast<uint4 *>(out + lane * 128 + (((h + e) ^ (lane & 7)) << 4)) =
-                                make_uint4(pack_bf16(o[8 * e], o[8 * e + 1]), pack_bf16(o[8 * e + 2], o[8 * e + 3]),
-                                           pack_bf16(o[8 * e + 4], o[8 * e + 5]), pack_bf16(o[8 * e + 6], o[8 * e + 7]));
-                        if (c & 32) leave((c - 32) * 2);
+                            for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(o[e + k] * inv);
+                            store32(po + c + e, w, true);
+                        }
+                    } else if (used) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 16) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) w[k] = pack_bf16(o[e + 2 * k] * inv, o[e + 2 * k + 1] * inv);
+                            store32(bo + c + e, w, wide);
+                        }
                     }
                 }
+                __syncwarp();
                 if (used) {
+                    const float l2 = sum == 0.f ? -INFINITY : top * g.c2 + log2f(sum);
                     if (split) g.parts.lse[g.parts.row(u.chunk, row, head)] = l2;
                     else if (a.lse) a.lse[row * a.H + head] = l2 * LN2;
                 }
             }
-            if (used && g.parts.count && u.chunk == 0 && head == 0) g.parts.count[row] = u.chunks;
+            if (PAGED && used && g.parts.count && u.chunk == 0 && head == 0) g.parts.count[row] = u.chunks;
             tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bars + 8 * (U_EMPTY + (i & 3)));
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -605,14 +742,14 @@ auto exponentials = [&](auto poly) {  // pairs of each eight that go by polynomi
                         const int t = u.t0 + y * g.tok;
                         int end = t >= u.live ? 0 : stop;
                         if (!(PAGED && a.parent)) end = min(end, cached + t + g.tok);
-                        const int tiles = max(end - u.kbeg + KEYS - 1, 0) / KEYS;
-                        (y ? u.n1 : u.n0) = tiles;
+                        const int halves = max(end - u.kbeg + HALF - 1, 0) / HALF;
+                        (y ? u.n1 : u.n0) = halves;
                     }
                 }
-                if (i >= 2 && !wait(&bar.u_empty[i & 1], ((i >> 1) - 1) & 1, abort)) break;
+                if (i >= 4 && !wait(bars + 8 * (U_EMPTY + (i & 3)), ((i >> 2) - 1) & 1, abort)) break;
                 if (lane == 0) {
-                    units[i & 1] = u;
-                    mbar_arrive(&bar.u_full[i & 1]);
+                    units[i & 3] = u;
+                    bar_arrive(bars + 8 * (U_FULL + (i & 3)));
                 }
                 __syncwarp();
             }
@@ -622,17 +759,17 @@ auto exponentials = [&](auto poly) {  // pairs of each eight that go by polynomi
             uint32_t it = 0, qn = 0;  // tiles and Q loads issued
             bool ok = true;
             for (int i = 0; ok && next_unit(i, u); ++i) {
-                const int tiles = max(u.n0, u.n1);
+                const int tiles = (max(u.n0, u.n1) + 1) / 2;
                 if (tiles == 0) continue;
-                if (qn > 0) ok = wait(&bar.q_empty, (qn - 1) & 1, abort);
+                if (qn > 0) ok = wait(bars + 8 * Q_EMPTY, (qn - 1) & 1, abort);
                 if (!ok) break;
                 if (lane == 0) {
                     const uint32_t bytes = static_cast<uint32_t>(g.tok * g.group) * D * 2;
-                    mbar_arrive_expect_tx(&bar.q_full, bytes * ((u.n0 > 0) + (u.n1 > 0)));
+                    bar_expect(bars + 8 * Q_FULL, bytes * ((u.n0 > 0) + (u.n1 > 0)));
                     for (int x = 0; x < 2; ++x)
                         for (int h = 0; (x ? u.n1 : u.n0) > 0 && h < C::HALVES; ++h)
-                            tma_load_3d(smem + C::OFF_Q + x * C::TILE + h * 16384, &tm_q, h * 64, u.kvh * g.group,
-                                        u.first + u.t0 + x * g.tok, &bar.q_full);
+                            load_3d(base + C::OFF_Q + x * C::TILE + h * 16384, &tm_q, h * 64, u.kvh * g.group,
+                                        u.first + u.t0 + x * g.tok, bars + 8 * Q_FULL);
                 }
                 ++qn;
                 const int rows = g.rows, pages = KEYS / rows;
@@ -653,11 +790,11 @@ auto exponentials = [&](auto poly) {  // pairs of each eight that go by polynomi
                     for (int kv = 0; kv < 2; ++kv, ++it) {
                         const int st = it % C::STAGES;
                         const uint32_t lap = it / C::STAGES;
-                        if (lap > 0 && !wait(&bar.kv_empty[st], (lap - 1) & 1, abort)) {
+                        if (lap > 0 && !wait(bars + 8 * (KV_EMPTY + st), (lap - 1) & 1, abort)) {
                             ok = false;
                             break;
                         }
-                        char *dst = smem + C::OFF_KV + st * C::TILE;
+                        const uint32_t dst = base + C::OFF_KV + st * C::TILE;
                         const CUtensorMap *tm = kv ? &tm_v : &tm_k;
                         if (PAGED) {
                             if (kv == 1 && lane < 4) {  // which of the tile's keys have memory behind them
@@ -666,117 +803,128 @@ auto exponentials = [&](auto poly) {  // pairs of each eight that go by polynomi
                                     w = 0;
                                     for (int b = 0; b < 32; ++b) w |= (valid >> ((lane * 32 + b) / rows) & 1u) << b;
                                 }
-                                masks[st][lane] = w;
+                                sts(masks + 16 * st + 4 * lane, w);
                             }
                             __syncwarp();
-                            if (lane == 0) mbar_arrive_expect_tx(&bar.kv_full[st], __popc(valid) * rows * D * 2);
+                            if (lane == 0) bar_expect(bars + 8 * (KV_FULL + st), __popc(valid) * rows * D * 2);
                             __syncwarp();
                             if (there)
                                 for (int h = 0; h < C::HALVES; ++h)
-                                    asm volatile(
-                                        "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-                                            smem_u32(dst + h * 16384 + lane * rows * 128)),
-                                        "l"(reinterpret_cast<uint64_t>(tm)), "r"(h * 64), "r"(at), "r"(smem_u32(&bar.kv_full[st]))
-                                        : "memory");
+                                    load_2d(dst + h * 16384 + lane * rows * 128, tm, h * 64, at, bars + 8 * (KV_FULL + st));
                         } else if (lane == 0) {
-                            mbar_arrive_expect_tx(&bar.kv_full[st], C::TILE);
+                            bar_expect(bars + 8 * (KV_FULL + st), C::TILE);
                             for (int h = 0; h < C::HALVES; ++h)
-                                tma_load_3d(dst + h * 16384, tm, h * 64, u.kvh, u.first + key, &bar.kv_full[st]);
+                                load_3d(dst + h * 16384, tm, h * 64, u.kvh, u.first + key, bars + 8 * (KV_FULL + st));
                         }
                         __syncwarp();
                     }
                 }
             }
-            if (*abort) {  // copies in flight land before the CTA leaves
+            if (lds(abort)) {  // copies in flight land before the CTA leaves
                 for (uint32_t k = it > C::STAGES ? it - C::STAGES : 0; k < it; ++k)
-                    mbar_wait(&bar.kv_full[k % C::STAGES], (k / C::STAGES) & 1, 1000000000ull);
-                if (qn > 0) mbar_wait(&bar.q_full, (qn - 1) & 1, 1000000000ull);
+                    drain_wait(bars + 8 * (KV_FULL + (k % C::STAGES)), (k / C::STAGES) & 1);
+                if (qn > 0) drain_wait(bars + 8 * Q_FULL, (qn - 1) & 1);
             }
-        } else if (warp == WARP_MMA) {
-            Unit u;
-            uint32_t it = 0, qn = 0, pn0 = 0, pn1 = 0;
-            bool ok = true;
-            for (int i = 0; ok && next_unit(i, u); ++i) {
-                const int tiles = max(u.n0, u.n1);
-                if (tiles == 0) continue;
-                if (lane == 0) {
-                    // A descriptor's address field counts 16 bytes: steps are added to it.
-                    const uint64_t dq = sdesc_sw128(base + C::OFF_Q, 16, 1024);
-                    const uint64_t dk = sdesc_sw128(base + C::OFF_KV, 16, 1024);
-                    const uint64_t dv = sdesc_sw128(base + C::OFF_KV, 16384, 1024);
-                    auto qk = [&](int x, int st) {
-                        const uint64_t qa = dq + x * (C::TILE >> 4), ka = dk + st * (C::TILE >> 4);
+        } else if (warp < WARP_TMA) {
+            // Products of row tile x. One thread per tile: a step's twelve products
+            // take one thread some 1,100 cycles to issue, as long as the tensor cores take for them.
+            // The warp stays together and its values are broadcast, so that they
+            // live in uniform registers, which the products take their operands from.
+            const int x = __shfl_sync(0xffffffffu, warp, 0) - WARP_MMA;
+            const bool chosen = elect_one();
+            // A descriptor's address field counts 16 bytes: steps are added to
+            // its low word (addresses stay below 2^18, so nothing carries).
+            const uint64_t like = sdesc_sw128(0, 16, 1024), like_v = sdesc_sw128(0, 16384, 1024);
+            const uint32_t hi = static_cast<uint32_t>(like >> 32), hi_v = static_cast<uint32_t>(like_v >> 32);
+            const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t q_lo = static_cast<uint32_t>(like) + ((base + C::OFF_Q + x * C::TILE) >> 4);
+            const uint32_t k_lo = static_cast<uint32_t>(like) + ((base + C::OFF_KV) >> 4);
+            const uint32_t v_lo = static_cast<uint32_t>(like_v) + ((base + C::OFF_KV) >> 4);
+            auto qk = [&](int h, int st) {
+                const uint32_t ka = k_lo + st * (C::TILE >> 4) + h * (HALF * 128 >> 4), d = t0 + x * 128 + h * HALF;
+                if (chosen) {
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {
-                            const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                            umma_f16(tmem + x * 128, qa + off, ka + off, C::ID_QK, k > 0);
-                        }
-                        umma_commit(&bar.s_full[x]);
-                    };
-                    auto pv = [&](int x, int st, int half, bool more) {
-                        const uint64_t va = dv + st * (C::TILE >> 4) + half * (8192 >> 4);
-                        const uint32_t p = tmem + x * 128 + half * 32;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_f16_ta(tmem + 256 + x * 128, p + 8 * k, va + k * (2048 >> 4), C::ID_PV, more || k + half > 0);
-                    };
-                ok = wait1(&bar.q_full, qn & 1, abort) && wait1(&bar.kv_full[it % C::STAGES], (it / C::STAGES) & 1, abort);
-                    if (ok) {
-#pragma unroll 1
-                        for (int x = 0; x < 2; ++x)
-                            if ((x ? u.n1 : u.n0) > 0) qk(x, it % C::STAGES);
-                        umma_commit(&bar.kv_empty[it % C::STAGES]);
-                        if (tiles == 1) umma_commit(&bar.q_empty);
-                        ++it;
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                        mma_ss(d, q_lo + off, ka + off, hi, C::ID_QK, k > 0);
                     }
-                    for (int j = 0; ok && j < tiles; ++j) {
-                        const int vs = it % C::STAGES;
-                        const uint32_t kt = it + 1;
-                        const int ks = kt % C::STAGES;
-                        ok = wait1(&bar.kv_full[vs], (it / C::STAGES) & 1, abort);
-                        bool have_k = false;
-#pragma unroll 1
-                        for (int x = 0; ok && x < 2; ++x) {
-                            const int n = x ? u.n1 : u.n0;
-                            if (j < n) {
-                                uint32_t &pn = x ? pn1 : pn0;
-#pragma unroll 1
-                                for (int half = 0; ok && half < 2; ++half) {
-                                    ok = wait1(&bar.p_full[x][half], pn & 1, abort);
-                                    if (!ok) break;
-                                    tc_fence_after();
-                                    pv(x, vs, half, j > 0);
-                                }
-                                if (!ok) break;
-                                ++pn;
-                                if (j + 1 == n) umma_commit(&bar.o_full[x]);
-                            }
-                            if (j + 1 < n) {
-                                if (!have_k) {
-                                    ok = wait1(&bar.kv_full[ks], (kt / C::STAGES) & 1, abort);
-                                    if (!ok) break;
-                                    have_k = true;
-                                }
-                                qk(x, ks);
-                            }
-                        }
-                        if (!ok) break;
-                        umma_commit(&bar.kv_empty[vs]);
-                        if (j + 1 < tiles) {
-                            umma_commit(&bar.kv_empty[ks]);
-                            if (j + 2 == tiles) umma_commit(&bar.q_empty);
-                            it += 2;
-                        } else {
-                            it += 1;
-                        }
-                    }
+                    commit(bars + 8 * (S_FULL + 2 * x + h));
                 }
+                __syncwarp();
+            };
+            auto pv = [&](int h, int st, bool more) {
+                const uint32_t va = v_lo + st * (C::TILE >> 4) + h * (HALF * 128 >> 4);
+                const uint32_t p = t0 + x * 128 + h * HALF, d = t0 + 256 + x * 128;
+                if (chosen) {
+#pragma unroll
+                    for (int k = 0; k < HALF / 16; ++k) mma_ts(d, p + 8 * k, va + k * (2048 >> 4), hi_v, C::ID_PV, more || k > 0);
+                    commit(bars + 8 * (PV_DONE + x));
+                }
+                __syncwarp();
+            };
+            auto done = [&](uint32_t bar) {  // arrives when every product so far is done
+                if (chosen) commit(bar);
+                __syncwarp();
+            };
+            Unit u;
+            uint32_t it = 0, qn = 0, pp = 0;  // pp: phases of P_FULL waited for, one bit per half
+            bool ok = true;
+#pragma unroll 1
+            for (int i = 0; ok && next_unit(i, u); ++i) {
+                const int tiles = __shfl_sync(0xffffffffu, (max(u.n0, u.n1) + 1) / 2, 0);
+                const int n = __shfl_sync(0xffffffffu, x ? u.n1 : u.n0, 0);
+                if (tiles == 0) continue;
+                int st = it % C::STAGES;
+                uint32_t lap = it / C::STAGES;
+                ok = wait(bars + 8 * Q_FULL, qn & 1, abort) && wait(bars + 8 * (KV_FULL + st), lap & 1, abort);
+                if (!ok) break;
+                if (n > 0) qk(0, st);
+                if (n > 1) qk(1, st);
+                done(bars + 8 * (KV_EMPTY + st));
+                if (tiles == 1) done(bars + 8 * Q_EMPTY);
+#pragma unroll 1
+                for (int j = 0; j < tiles; ++j) {
+                    // V of this key tile, K of the next.
+                    const int vs = st + 1 == C::STAGES ? 0 : st + 1, ks = vs + 1 == C::STAGES ? 0 : vs + 1;
+                    const uint32_t vlap = lap + (vs < st), klap = vlap + (ks < vs);
+                    // (Also where this row tile has no use for them: an arrival on
+                    // KV_EMPTY belongs to the lap whose KV_FULL it follows.)
+                    ok = wait(bars + 8 * (KV_FULL + vs), vlap & 1, abort);
+                    if (!ok) break;
+                    bool have_k = false;
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        const int e = 2 * j + h;  // P of this half is there: its product, then the scores that take its place
+                        if (e < n) {
+                            ok = wait(bars + 8 * (P_FULL + 2 * x + h), pp >> h & 1, abort);
+                            if (!ok) break;
+                            pp ^= 1u << h;
+                            tc_fence_after();
+                            pv(h, vs, e > 0);
+                            if (e + 1 == n) done(bars + 8 * (O_FULL + x));
+                        }
+                        if (j + 1 < tiles && !have_k) {
+                            ok = wait(bars + 8 * (KV_FULL + ks), klap & 1, abort);
+                            if (!ok) break;
+                            have_k = true;
+                        }
+                        if (e + 2 < n) qk(h, ks);
+                    }
+                    if (!ok) break;
+                    done(bars + 8 * (KV_EMPTY + vs));
+                    if (j + 1 < tiles) {
+                        done(bars + 8 * (KV_EMPTY + ks));
+                        if (j + 2 == tiles) done(bars + 8 * Q_EMPTY);
+                    }
+                    st = ks;
+                    lap = klap;
+                }
+                it += 2 * tiles;
                 ++qn;
-                ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
             }
-            if (*abort && lane == 0) {  // products in flight finish before TMEM is freed
-                umma_commit(&bar.drain);
-                mbar_wait(&bar.drain, 0, 1000000000ull);
+            if (lds(abort) && chosen) {  // products in flight finish before TMEM is freed
+                commit(bars + 8 * DRAIN);
+                drain_wait(bars + 8 * DRAIN, 0);
             }
             __syncwarp();
         }
