@@ -25,7 +25,6 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
-#include <type_traits>
 
 #include "attn_common.cuh"
 #include "sm100.cuh"
@@ -43,10 +42,7 @@ constexpr int HALF = 64;    // keys of a step
 constexpr int THREADS = 384;
 constexpr int WARP_MMA = 8, WARP_TMA = 10, WARP_SCHED = 11;  // (two of the first)
 constexpr int GROUP = 256;  // sequences whose unit counts the scheduler holds at a time
-#ifndef POLY_
-#define POLY_ 0
-#endif
-constexpr int POLY = POLY_;      // of 8 pairs of exponentials, so many by polynomial
+constexpr float FREE = 65536.f;  // probabilities may reach this against a maximum that was not looked for
 constexpr float LAZY = 8.f; // a row's maximum may grow by 2^LAZY before O is rescaled
 
 // Sticky: a bounded wait of this kernel ran out.
@@ -66,10 +62,11 @@ template <int D>
 struct Cfg {
     static constexpr int HALVES = D / 64;
     static constexpr int TILE = KEYS * D * 2;              // a K, V or Q tile in bytes
-    static constexpr int STAGES = D == 128 ? 5 : 8;        // K and V tiles in flight
+    static constexpr int STAGES = D == 128 ? 4 : 8;        // K and V tiles in flight
     static constexpr int OFF_Q = 0;
     static constexpr int OFF_KV = 2 * TILE;
-    static constexpr int OFF_BAR = OFF_KV + STAGES * TILE; // barriers, units, scheduler's counts
+    static constexpr int OFF_OUT = OFF_KV + STAGES * TILE; // 4 KB per softmax warp: output rows on their way out
+    static constexpr int OFF_BAR = OFF_OUT + 8 * 4096;     // barriers, units, scheduler's counts
     static constexpr int OFF_UNIT = OFF_BAR + 320;
     static constexpr int OFF_MASK = OFF_UNIT + 256;
     static constexpr int OFF_MISC = OFF_MASK + 128;
@@ -150,6 +147,17 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_l
         "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(more))
         : "memory");
 }
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -224,29 +232,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// 2^x without the special-function unit, two at once: x = n + f with n the
-// nearest integer (the low bits of x + 1.5 * 2^23), |f| <= 1/2, then a
-// degree-5 polynomial in f (least maximal relative error among those with
-// constant term 1: 2^-22.4 in f32 arithmetic, as close as ex2.approx) and n
-// added to the exponent. x is held at -127, where f = 0 and the sum of
-// exponents is exactly 0.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-    constexpr float MAGIC = 12582912.f;
-    x.x = fmaxf(x.x, -127.f);
-    x.y = fmaxf(x.y, -127.f);
-    const float2 t = add2(x, make_float2(MAGIC, MAGIC));
-    const float2 n = add2(t, make_float2(-MAGIC, -MAGIC));
-    const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
-    float2 p = make_float2(0.001326472731307149f, 0.001326472731307149f);
-    p = fma2(p, f, make_float2(0.009671512991189957f, 0.009671512991189957f));
-    p = fma2(p, f, make_float2(0.05550733581185341f, 0.05550733581185341f));
-    p = fma2(p, f, make_float2(0.24022242426872253f, 0.24022242426872253f));
-    p = fma2(p, f, make_float2(0.6931470036506653f, 0.6931470036506653f));
-    p = fma2(p, f, make_float2(1.f, 1.f));
-    return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(p.x)),
-                       __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(p.y)));
-}
-
 // 8 consecutive 32-bit columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -270,20 +255,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// 32 bytes of a row: one store where the address allows it.
-__device__ __forceinline__ void store32(void *p, const uint32_t (&w)[8], bool wide) {
-    if (wide) {
-        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                     "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                     : "memory");
-    } else {
-        static_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        static_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-    }
-}
-
-__device__ __forceinline__ bool aligned32(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
-
 // Bits of the 32 keys from `start` that a row sees (`all`: keys below it are
 // seen; `bits`: the 64 keys from `all` on).
 __device__ __forceinline__ uint32_t seen_word(int all, uint64_t bits, int start) {
@@ -291,6 +262,39 @@ __device__ __forceinline__ uint32_t seen_word(int all, uint64_t bits, int start)
     if (n >= 32) return ~0u;
     if (n > 0) return ((1u << n) - 1u) | static_cast<uint32_t>(bits << n);
     return n > -64 ? static_cast<uint32_t>(bits >> -n) : 0u;
+}
+
+// V of a step that not every row sees whole, a step's 64 keys by a warpgroup,
+// two threads to a key: rows behind the sequence or without a page become
+// zero, and values that are not finite in rows from key `full` on are noted
+// at `spoiled`. (A probability of zero does not keep them out of a product.)
+template <int D, bool PAGED>
+__device__ __forceinline__ void clean_values(uint32_t tile, uint32_t mask, int h, int key, int keys, int full, int r,
+                                             uint32_t spoiled, int mark) {
+    const int kr = r >> 1;
+    const uint32_t vrow = tile + (h * HALF + kr) * 128 + (D == 128 ? (r & 1) * 16384 : 0);
+    const bool exists = key + kr < keys && (!PAGED || (lds(mask + 8 * h + 4 * (kr >> 5)) >> (kr & 31) & 1u));
+    if (!exists || key + kr >= full) {
+        bool bad = false;
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {  // 16-byte pieces; lanes start at different ones: different banks
+            const int piece = D == 128 ? ((c + kr) & 7) : ((c + kr) & 3) + 4 * (r & 1);
+            const uint32_t at = vrow + piece * 16;
+            if (!exists) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+            } else {
+                uint32_t ws[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(ws[0]), "=r"(ws[1]), "=r"(ws[2]), "=r"(ws[3])
+                             : "r"(at)
+                             : "memory");
+#pragma unroll
+                for (int k = 0; k < 4; ++k) bad |= (ws[k] & 0x7f80u) == 0x7f80u || (ws[k] & 0x7f800000u) == 0x7f800000u;
+            }
+        }
+        if (bad) sts(spoiled, mark);
+    }
+    fence_proxy_async_smem();
 }
 
 // One row by plain arithmetic from global memory, a warp per row: for tiles
@@ -416,30 +420,41 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + 256 + x * 128;
         uint32_t sn = 0, on = 0, it = 0;  // steps and units done (mod 2^32) of this row tile, ring position of the unit's first tile
         uint32_t sp = 0;          // phases of S_FULL waited for, one bit per half
+        const int row_token = r / g.group, row_head = r - row_token * g.group;
         for (int i = 0; wait(bars + 8 * (U_FULL + (i & 3)), (i >> 2) & 1, abort); ++i) {
             const Unit &u = units[i & 3];
             if (!u.valid) break;
+            const int token = u.t0 + x * g.tok + row_token;
+            const bool used = row_token < g.tok && token < u.m;
             int all = 0;         // what the row sees: keys below `all`, and of the 64 from there on those in `bits`
             uint64_t bits = 0;
-            {
-                const int token = u.t0 + x * g.tok + r / g.group;
-                if (r < g.tok * g.group && token < u.m) {
-                    Seq s;
-                    s.first = u.first; s.m = u.m; s.live = u.live; s.cached = u.cached; s.keys = u.keys;
-                    const Sight sight = sight_of(a, s, token);
-                    all = static_cast<int>(sight.all);
-                    if (PAGED) bits = sight.bits;
+            if (used && token < u.live) {
+                if (PAGED && a.parent) {
+                    bits = ancestors(a.parent + u.first, token);
+                    all = bits ? u.cached : 0;
+                } else {
+                    all = u.cached + token + 1;
                 }
             }
             // Tiles below `full` are seen whole by every live row of the warpgroup's tile.
             const int full = PAGED && a.parent ? u.cached : u.cached + u.t0 + x * g.tok + 1;
             const int kbeg = u.kbeg;
+            const bool sees = all > 0 || bits != 0;  // (rows that do not are computed and thrown away)
             float top = -INFINITY, sum = 0.f;
             bool ok = true;
             const int n = x ? u.n1 : u.n0;
+            // Halves that every live row sees whole.
+            const int whole = min(max(full - kbeg, 0) / HALF, n);
+            bool loaded = false;  // v holds step e's scores
+            float v[2][32];
+            auto load = [&](int h) {
+                tc_fence_after();
+#pragma unroll
+                for (int w = 0; w < 2; ++w) tmem_ld32(ts + HALF * h + 32 * w, v[w]);
+            };
             for (int e = 0; e < n; ++e, ++sn) {
                 const int h = e & 1, key = kbeg + e * HALF;
-                bool edge = key + HALF > full;
+                bool edge = e >= whole;
                 uint32_t there[2] = {~0u, ~0u};
                 if (PAGED || edge) {
                     const uint32_t vt = it + (e | 1);  // this tile's V in the ring
@@ -453,88 +468,24 @@ __global__ void __launch_bounds__(THREADS, 1)
                             edge |= there[w] != ~0u;
                         }
                     }
-                    if (edge) {
-                        // V: rows behind the sequence or without a page become zero,
-                        // values that are not finite in rows not everyone sees are
-                        // noted. Two threads to a key's row.
-                        const int kr = r >> 1;
-                        const uint32_t vrow = base + C::OFF_KV + vs * C::TILE + (h * HALF + kr) * 128 + (D == 128 ? (r & 1) * 16384 : 0);
-                        const bool exists = key + kr < u.keys && (!PAGED || (lds(masks + 16 * vs + 8 * h + 4 * (kr >> 5)) >> (kr & 31) & 1u));
-                        if (!exists || key + kr >= full) {
-                            bool bad = false;
-#pragma unroll 2
-                            for (int c = 0; c < D / 16; ++c) {  // 16-byte pieces; lanes start at different ones: different banks
-                                const int piece = D == 128 ? ((c + (lane >> 1)) & 7) : ((c + (lane >> 1)) & 3) + 4 * (r & 1);
-                                const uint32_t at = vrow + piece * 16;
-                                if (!exists) {
-                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                                } else {
-                                    uint32_t ws[4];
-                                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                                 : "=r"(ws[0]), "=r"(ws[1]), "=r"(ws[2]), "=r"(ws[3])
-                                                 : "r"(at)
-                                                 : "memory");
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k)
-                                        bad |= (ws[k] & 0x7f80u) == 0x7f80u || (ws[k] & 0x7f800000u) == 0x7f800000u;
-                                }
-                            }
-                            if (bad) sts(spoiled + 16 * x + 4 * (i & 3), i + 1);
-                        }
-                        fence_proxy_async_smem();
-                    }
+                    if (edge) clean_values<D, PAGED>(base + C::OFF_KV + vs * C::TILE, masks + 16 * vs, h, key, u.keys, full, r, spoiled + 16 * x + 4 * (i & 3), i + 1);
                 }
-                ok = wait(bars + 8 * (S_FULL + 2 * x + h), sp >> h & 1, abort);
-                if (!ok) break;
-                sp ^= 1u << h;
-                tc_fence_after();
-                float v[2][32];
-#pragma unroll
-                for (int w = 0; w < 2; ++w) tmem_ld32(ts + HALF * h + 32 * w, v[w]);
-                tmem_wait_ld();
-                if (edge) {
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const uint32_t m = seen_word(all, bits, key + 32 * w) & there[w];
-                        if (m != ~0u) {
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) v[w][k] = m >> k & 1u ? v[w][k] : -INFINITY;
-                        }
-                    }
-                }
-                float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int k = 0; k < 32; k += 4)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) best[w] = max3(best[w], v[w >> 1][k + 2 * (w & 1)], v[w >> 1][k + 2 * (w & 1) + 1]);
-                const float peak = fmaxf(max3(best[0], best[1], best[2]), best[3]);
-                if (e == 0) {
-                    top = peak;
-                } else if (__any_sync(0xffffffffu, (peak - top) * g.c2 > LAZY)) {
-                    const float now = fmaxf(top, peak);
-                    const float keep = now == top ? 1.f : ex2((top - now) * g.c2);
-                    top = now;
-                    sum *= keep;
-                    // O holds every step before this one (that step sn - 2 is done follows
-                    // from S, so the parity tells step sn - 1 from it)
-                    ok = wait(bars + 8 * (PV_DONE + x), (sn - 1) & 1, abort);
+                if (!loaded) {
+                    ok = wait(bars + 8 * (S_FULL + 2 * x + h), sp >> h & 1, abort);
                     if (!ok) break;
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 8) {  // few registers: the scores are held meanwhile
-                        uint32_t o[8];
-                        tmem_ld8(to + c, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                        tmem_st8(to + c, o);
-                    }
+                    load(h);
+                    tmem_wait_ld();
                 }
-                const float from = top == -INFINITY ? 0.f : -top * g.c2;
-                const float2 c2 = make_float2(g.c2, g.c2), f2 = make_float2(from, from);
-                float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                auto exponentials = [&](auto poly) {  // pairs of each eight that go by polynomial
-                    uint32_t p[32];
+                sp ^= 1u << h;
+                loaded = false;
+                const float2 c2 = make_float2(g.c2, g.c2);
+                float2 part[2];
+                uint32_t p[32];
+                // p = exp2(c s - c top) and its sum.
+                auto exponentials = [&]() {
+                    const float from = top == -INFINITY ? 0.f : -top * g.c2;
+                    const float2 f2 = make_float2(from, from);
+                    part[0] = part[1] = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int b = 0; b < 32; b += 8) {
                         float2 y[8];
@@ -545,12 +496,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                         }
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            if (k < decltype(poly)::value) {
-                                y[k] = ex2_poly(y[k]);
-                            } else {
-                                y[k].x = ex2(y[k].x);
-                                y[k].y = ex2(y[k].y);
-                            }
+                            y[k].x = ex2(y[k].x);
+                            y[k].y = ex2(y[k].y);
                         }
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
@@ -558,16 +505,73 @@ __global__ void __launch_bounds__(THREADS, 1)
                             p[b + k] = pack_bf16(y[k].x, y[k].y);
                         }
                     }
-                    tmem_st32u(ts + HALF * h, p);
+                    part[0] = add2(part[0], part[1]);
                 };
-                if (POLY == 0 || edge) exponentials(std::integral_constant<int, 0>{});  // masked scores give exact zeros
-                else exponentials(std::integral_constant<int, POLY>{});
+                // Without looking for the maximum first: against the one in use
+                // no probability of these 64 is above 2^FREE if their sum is not
+                // (the search took 280 of a step's 1,900 cycles).
+                bool settled = false;
+                if (e > 0 && !edge) {
+                    exponentials();
+                    settled = __all_sync(0xffffffffu, !sees || (part[0].x + part[0].y <= FREE && top > -INFINITY));
+                    if (!settled) {
+                        load(h);
+                        tmem_wait_ld();
+                    }
+                }
+                if (!settled) {
+                    if (edge) {
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const uint32_t m = seen_word(all, bits, key + 32 * w) & there[w];
+                            if (m != ~0u) {
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) v[w][k] = m >> k & 1u ? v[w][k] : -INFINITY;
+                            }
+                        }
+                    }
+                    float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) best[w] = max3(best[w], v[w >> 1][k + 2 * (w & 1)], v[w >> 1][k + 2 * (w & 1) + 1]);
+                    const float peak = fmaxf(max3(best[0], best[1], best[2]), best[3]);
+                    if (e == 0) {
+                        top = peak;
+                    } else if (__any_sync(0xffffffffu, sees && (peak - top) * g.c2 > LAZY)) {
+                        const float now = fmaxf(top, peak);
+                        const float keep = now == top ? 1.f : ex2((top - now) * g.c2);
+                        top = now;
+                        sum *= keep;
+                        // O holds every step before this one (that step sn - 2 is done follows
+                        // from S, so the parity tells step sn - 1 from it)
+                        ok = wait(bars + 8 * (PV_DONE + x), (sn - 1) & 1, abort);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 8) {  // few registers: the scores are held meanwhile
+                            uint32_t o[8];
+                            tmem_ld8(to + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                            tmem_st8(to + c, o);
+                        }
+                    }
+                    exponentials();
+                }
+                tmem_st32u(ts + HALF * h, p);
+                // The next step's scores come while the probabilities go, if they are there already.
+                if (e + 1 < n && __all_sync(0xffffffffu, bar_test(bars + 8 * (S_FULL + 2 * x + (h ^ 1)), sp >> (h ^ 1) & 1))) {
+                    load(h ^ 1);
+                    loaded = true;
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(bars + 8 * (P_FULL + 2 * x + h));
-                part[0] = add2(part[0], part[1]);
                 sum += part[0].x + part[0].y;
+                if (loaded) tmem_wait_ld();
             }
             if (!ok) break;
             it += 2 * ((max(u.n0, u.n1) + 1) / 2);
@@ -578,12 +582,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc_fence_after();
                 bad = lds(spoiled + 16 * x + 4 * (i & 3)) == i + 1;  // written before its warp's last p_full arrival
             }
-            const bool blind = all == 0 && bits == 0;  // sees nothing: whole tiles above did not ask
-            if (blind) sum = 0.f;
-            const int token = u.t0 + x * g.tok + r / g.group;
-            const bool used = r < g.tok * g.group && token < u.m;
+            if (!sees) sum = 0.f;
             const int64_t row = u.first + token;
-            const int head = u.kvh * g.group + r % g.group;
+            const int head = u.kvh * g.group + row_head;
             const bool split = PAGED && u.chunks > 1;
             if (bad) {
                 const int kend = min(u.keys, u.kbeg + n * HALF);
@@ -594,42 +595,61 @@ __global__ void __launch_bounds__(THREADS, 1)
                         plain_row<D, PAGED>(g, u, x * g.tok * g.group + rr, theirs, kend, lane);
                 }
             } else {
-                // A thread writes its row's 32 bytes at a time: whole sectors.
+                // Rows leave through the warp's 4 KB of shared memory, 128 bytes of
+                // each at a time, so that eight lanes write a row's whole line: a
+                // thread that writes its own row touches 32 lines per store, and the
+                // 64 KB of a unit took 2,900 cycles that way.
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                float *po = g.parts.o + g.parts.row(u.chunk, row, head) * D;
-                __nv_bfloat16 *bo = static_cast<__nv_bfloat16 *>(a.o) + (row * a.H + head) * D;
-                const bool wide = aligned32(a.o);
+                const uint32_t mine = used ? static_cast<uint32_t>(split ? g.parts.row(0, row, head) : row * a.H + head) : ~0u;
+                const uint32_t out = base + C::OFF_OUT + warp * 4096;
+                char *dst = (split ? reinterpret_cast<char *>(g.parts.o + g.parts.row(u.chunk, 0, 0) * D) : static_cast<char *>(a.o)) + (lane & 7) * 16;
+                const int row_bytes = split ? D * 4 : D * 2;
+                auto put = [&](int piece, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((piece ^ (lane & 7)) << 4)),
+                                 "r"(w0), "r"(w1), "r"(w2), "r"(w3)
+                                 : "memory");
+                };
+                uint32_t to_row[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) to_row[k] = __shfl_sync(0xffffffffu, mine, 4 * k + (lane >> 3));
+                auto leave = [&](int at) {  // 128 bytes of every row, from byte `at` of the row
+                    __syncwarp();
+                    uint4 q[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(q[k].x), "=r"(q[k].y), "=r"(q[k].z), "=r"(q[k].w)
+                                     : "r"(out + (4 * k + (lane >> 3)) * 128 + (((lane & 7) ^ ((4 * k + (lane >> 3)) & 7)) << 4)));
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (to_row[k] != ~0u) *reinterpret_cast<uint4 *>(dst + static_cast<int64_t>(to_row[k]) * row_bytes + at) = q[k];
+                };
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     float o[32];
-                    __syncwarp();
                     if (n > 0) {
                         tmem_ld32(to + c, o);
                         tmem_wait_ld();
                     }
-                    if (n == 0 || blind) {
+                    if (n == 0 || !sees) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e) o[e] = 0.f;
                     }
-                    if (used && split) {
+                    if (split) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint32_t w[8];
+                        for (int e = 0; e < 8; ++e)
+                            put(e, __float_as_uint(o[4 * e] * inv), __float_as_uint(o[4 * e + 1] * inv),
+                                __float_as_uint(o[4 * e + 2] * inv), __float_as_uint(o[4 * e + 3] * inv));
+                        leave(c * 4);
+                    } else {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(o[e + k] * inv);
-                            store32(po + c + e, w, true);
-                        }
-                    } else if (used) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 16) {
-                            uint32_t w[8];
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) w[k] = pack_bf16(o[e + 2 * k] * inv, o[e + 2 * k + 1] * inv);
-                            store32(bo + c + e, w, wide);
-                        }
+                        for (int e = 0; e < 4; ++e)
+                            put((c >> 3 & 4) + e, pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+                        if (c & 32) leave((c - 32) * 2);
                     }
                 }
-                __syncwarp();
                 if (used) {
                     const float l2 = sum == 0.f ? -INFINITY : top * g.c2 + log2f(sum);
                     if (split) g.parts.lse[g.parts.row(u.chunk, row, head)] = l2;
@@ -878,8 +898,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 uint32_t lap = it / C::STAGES;
                 ok = wait(bars + 8 * Q_FULL, qn & 1, abort) && wait(bars + 8 * (KV_FULL + st), lap & 1, abort);
                 if (!ok) break;
-                if (n > 0) qk(0, st);
-                if (n > 1) qk(1, st);
+#pragma unroll 1
+                for (int h = 0; h < min(n, 2); ++h) qk(h, st);
                 done(bars + 8 * (KV_EMPTY + st));
                 if (tiles == 1) done(bars + 8 * Q_EMPTY);
 #pragma unroll 1
