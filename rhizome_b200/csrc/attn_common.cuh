@@ -147,5 +147,9 @@ __device__ __forceinline__ Sight sight_of(const AttnArgs &a, const Seq &s, int64
 bool attn_tc_supports(const AttnArgs &a);
 int launch_attn_tc(const AttnArgs &a, const attn::Parts &parts, attn::Split split);
 int attn_tc_status(int *flag, bool clear);
+// The form for few rows per sequence over the paged cache (attn_rows.cu).
+bool attn_rows_supports(const AttnArgs &a);
+int launch_attn_rows(const AttnArgs &a, const attn::Parts &parts, attn::Split split);
+int attn_rows_status(int *flag, bool clear);
 
 }  // namespace rhz

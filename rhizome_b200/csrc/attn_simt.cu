@@ -23,7 +23,7 @@ using namespace attn;
 
 constexpr int THREADS = 256;
 constexpr int KEYS = 64;                       // keys per tile
-constexpr Split SIMT_SPLIT{256, 64}, TC_SPLIT{2048, 64};
+constexpr Split SIMT_SPLIT{256, 64}, ROWS_SPLIT{256, 64}, TC_SPLIT{2048, 64};
 
 // Four consecutive elements as f32 (d % 4 == 0, 16-byte aligned bases).
 __device__ __forceinline__ float4 get4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
@@ -380,7 +380,9 @@ int launch_simt(const AttnArgs &a, const Parts &parts, Split split) {
     return few ? launch_simt_r<float, 16>(a, parts, split) : launch_simt_r<float, 64>(a, parts, split);
 }
 
-Split split_of(const AttnArgs &a) { return attn_tc_supports(a) ? TC_SPLIT : SIMT_SPLIT; }
+Split split_of(const AttnArgs &a) {
+    return attn_rows_supports(a) ? ROWS_SPLIT : attn_tc_supports(a) ? TC_SPLIT : SIMT_SPLIT;
+}
 
 int64_t chunk_bound(const AttnArgs &a) {
     return a.paged ? split_of(a).bound(a.width << a.shift) : 1;
@@ -398,12 +400,21 @@ int launch_attn(const AttnArgs &a) {
     const Parts parts = parts_at(a.ws, a.total_tokens, a.H, a.d, chunks);
     const Split split = split_of(a);
     // A cache of no pages has no tensor map; nothing is seen there.
-    const bool tc = attn_tc_supports(a) && !(a.paged && a.num_blocks == 0);
-    const int st = tc ? launch_attn_tc(a, parts, split) : launch_simt(a, parts, split);
+    const bool none = a.paged && a.num_blocks == 0;
+    const int st = none                    ? launch_simt(a, parts, split)
+                   : attn_rows_supports(a) ? launch_attn_rows(a, parts, split)
+                   : attn_tc_supports(a)   ? launch_attn_tc(a, parts, split)
+                                           : launch_simt(a, parts, split);
     if (st != RHZ_OK || chunks <= 1) return st;
     return launch_join(a, parts);
 }
 
-int attn_status(int *flag, bool clear) { return attn_tc_status(flag, clear); }
+int attn_status(int *flag, bool clear) {
+    int x = 0, y = 0;
+    int st = attn_tc_status(&x, clear);
+    if (st == RHZ_OK) st = attn_rows_status(&y, clear);
+    *flag = x | y;
+    return st;
+}
 
 }  // namespace rhz

@@ -27,6 +27,7 @@
 #include <cstdint>
 
 #include "attn_common.cuh"
+#include "attn_device.cuh"
 #include "sm100.cuh"
 #include "tmap.h"
 
@@ -97,26 +98,6 @@ struct TcArgs {
     float c2;    // scale * log2 e
 };
 
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"  // suspended for about 1 us at most
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
 __device__ __forceinline__ bool elect_one() {
     uint32_t one;
     asm volatile(
@@ -147,41 +128,9 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_l
         "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(more))
         : "memory");
 }
-__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ uint32_t lds(uint32_t at) {
-    uint32_t x;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
-    return x;
-}
-__device__ __forceinline__ void sts(uint32_t at, uint32_t x) {
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(x) : "memory");
-}
-__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap *tm, int c0, int c1, int c2, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap *tm, int c0, int c1, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(bar)
-        : "memory");
-}
-
 // Bounded wait of one thread (2^21 tries, some 0.1 to 2 s) that also ends when
 // another role gave up; *stop in shared memory tells the others.
 __device__ __forceinline__ bool wait1(uint32_t bar, uint32_t parity, uint32_t stop) {
@@ -206,12 +155,6 @@ __device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
 // The same for a whole warp: all its lanes go on or none does.
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t stop) {
     return __all_sync(0xffffffffu, wait1(bar, parity, stop));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 // (a * b + c) on two f32 at once.
@@ -250,20 +193,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
-
-// Bits of the 32 keys from `start` that a row sees (`all`: keys below it are
-// seen; `bits`: the 64 keys from `all` on).
-__device__ __forceinline__ uint32_t seen_word(int all, uint64_t bits, int start) {
-    const int n = all - start;  // keys of this word below `all`
-    if (n >= 32) return ~0u;
-    if (n > 0) return ((1u << n) - 1u) | static_cast<uint32_t>(bits << n);
-    return n > -64 ? static_cast<uint32_t>(bits >> -n) : 0u;
-}
-
 // V of a step that not every row sees whole, a step's 64 keys by a warpgroup,
 // two threads to a key: rows behind the sequence or without a page become
 // zero, and values that are not finite in rows from key `full` on are noted
@@ -295,56 +224,6 @@ __device__ __forceinline__ void clean_values(uint32_t tile, uint32_t mask, int h
         if (bad) sts(spoiled, mark);
     }
     fence_proxy_async_smem();
-}
-
-// One row by plain arithmetic from global memory, a warp per row: for tiles
-// that hold values which are not finite where some rows must not see them
-// (the tensor cores' 0 * NaN would reach every row of the tile).
-template <int D, bool PAGED>
-__device__ __noinline__ void plain_row(const TcArgs &g, const Unit &u, int row, const Sight &sight, int kend, int lane) {
-    constexpr int C = D / 32;  // channels of a lane
-    const AttnArgs &a = g.a;
-    const int64_t token = u.first + u.t0 + row / g.group;
-    const int head = u.kvh * g.group + row % g.group;
-    const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.q) + token * a.q_stride + static_cast<int64_t>(head) * D + lane * C;
-    float qx[C], acc[C], top = -INFINITY, sum = 0.f;
-    for (int e = 0; e < C; ++e) {
-        qx[e] = __bfloat162float(q[e]);
-        acc[e] = 0.f;
-    }
-    for (int key = u.kbeg; key < kend; ++key) {
-        if (!sight.sees(key)) continue;
-        int64_t kat, vat;
-        if (PAGED) {
-            const int64_t block = a.block_table[u.seq * a.width + (key >> a.shift)];
-            if (block < 0 || block >= a.num_blocks) continue;
-            kat = vat = (((block * a.Hkv + u.kvh) << a.shift) + (key & ((1 << a.shift) - 1))) * D;
-        } else {
-            kat = (static_cast<int64_t>(u.first) + key) * a.k_stride + static_cast<int64_t>(u.kvh) * D;
-            vat = (static_cast<int64_t>(u.first) + key) * a.v_stride + static_cast<int64_t>(u.kvh) * D;
-        }
-        float s = 0.f;
-        for (int e = 0; e < C; ++e) s = fmaf(qx[e], __bfloat162float(static_cast<const __nv_bfloat16 *>(a.k)[kat + lane * C + e]), s);
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        s *= g.c2;
-        const float best = fmaxf(top, s), from = best == -INFINITY ? 0.f : best;
-        const float keep = ex2(top - from), p = ex2(s - from);
-        top = best;
-        sum = sum * keep + p;
-        for (int e = 0; e < C; ++e)
-            acc[e] = fmaf(p, __bfloat162float(static_cast<const __nv_bfloat16 *>(a.v)[vat + lane * C + e]), acc[e] * keep);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const float l2 = sum == 0.f ? -INFINITY : top + log2f(sum);
-    if (u.chunks > 1) {
-        const int64_t r = g.parts.row(u.chunk, token, head);
-        if (lane == 0) g.parts.lse[r] = l2;
-        for (int e = 0; e < C; ++e) g.parts.o[r * D + lane * C + e] = acc[e] * inv;
-    } else {
-        if (lane == 0 && a.lse) a.lse[token * a.H + head] = l2 * LN2;
-        for (int e = 0; e < C; ++e)
-            static_cast<__nv_bfloat16 *>(a.o)[(token * a.H + head) * D + lane * C + e] = __float2bfloat16_rn(acc[e] * inv);
-    }
 }
 
 template <int D, bool PAGED>
@@ -592,7 +471,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const int rr = (warp & 3) * 32 + w;
                     const Sight theirs{__shfl_sync(0xffffffffu, all, w), __shfl_sync(0xffffffffu, bits, w)};
                     if (__shfl_sync(0xffffffffu, static_cast<int>(used), w))
-                        plain_row<D, PAGED>(g, u, x * g.tok * g.group + rr, theirs, kend, lane);
+                        plain_row<D>(a, g.parts, g.c2, {u.seq, u.kvh, u.first, u.kbeg, kend, u.chunk, u.chunks}, u.t0 + x * g.tok + rr / g.group,
+                                     rr % g.group, theirs, lane);
                 }
             } else {
                 // Rows leave through the warp's 4 KB of shared memory, 128 bytes of
