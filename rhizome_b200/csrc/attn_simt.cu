@@ -23,7 +23,7 @@ using namespace attn;
 
 constexpr int THREADS = 256;
 constexpr int KEYS = 64;                       // keys per tile
-constexpr Split SIMT_SPLIT{256, 64}, ROWS_SPLIT{256, 64}, TC_SPLIT{2048, 64};
+constexpr Split SIMT_SPLIT{256, 64}, ROWS_SPLIT{512, 64}, TC_SPLIT{2048, 64};
 
 // Four consecutive elements as f32 (d % 4 == 0, 16-byte aligned bases).
 __device__ __forceinline__ float4 get4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
@@ -284,11 +284,12 @@ __global__ void __launch_bounds__(THREADS) attn_simt_kernel(const AttnArgs a, co
 
 // Joins the chunks of a row: o = sum_c 2^(lse_c - lse) o_c in order of
 // position, one warp per (token, head). Rows of one chunk are final already.
-template <typename T>
+template <typename T, int FLIGHT>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, const Parts parts) {
     const int lane = threadIdx.x & 31;
     const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     const int64_t token = row / a.H;
+    cudaGridDependencySynchronize();  // launched early: the chunks' results are there from here on
     if (token >= a.total_tokens || token >= a.cu_seqlens[a.n_seq] || token < a.cu_seqlens[0]) return;
     const int head = static_cast<int>(row - token * a.H);
     const int chunks = min(parts.count[token], parts.most);
@@ -312,20 +313,31 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, const 
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
     const float inv = total == 0.f ? 0.f : 1.f / total;
+    // FLIGHT chunks' loads at a time: with four, 64 chunks of a row took a
+    // warp 39 us, sixteen round trips to memory (sixteen: 12 us); for many rows
+    // of few chunks, four leave room for more warps (27 us against 48 us for
+    // the rows of 48 trees).
     float acc[2][4] = {};
-#pragma unroll 4
-    for (int c = 0; c < chunks; ++c) {
-        const float w = __shfl_sync(0xffffffffu, c < 32 ? mine[0] : mine[1], c & 31);
-        const float *src = parts.o + parts.row(c, token, head) * a.d;
+    const float *src = parts.o + parts.row(0, token, head) * a.d + 4 * lane;
+    const int64_t next = parts.tokens * a.H * a.d;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const int col = 4 * lane + 128 * g;
-            if (col >= a.d) continue;
-            const float4 x = get4(src + col);
-            acc[g][0] = fmaf(w, x.x, acc[g][0]);
-            acc[g][1] = fmaf(w, x.y, acc[g][1]);
-            acc[g][2] = fmaf(w, x.z, acc[g][2]);
-            acc[g][3] = fmaf(w, x.w, acc[g][3]);
+    for (int g = 0; g < 2; ++g) {
+        const bool has = 4 * lane + 128 * g < a.d;
+        for (int c0 = 0; c0 < chunks && 128 * g < a.d; c0 += FLIGHT) {
+            float4 x[FLIGHT];
+#pragma unroll
+            for (int k = 0; k < FLIGHT; ++k)
+                if (has && c0 + k < chunks) x[k] = get4(src + (c0 + k) * next + 128 * g);
+#pragma unroll
+            for (int k = 0; k < FLIGHT; ++k) {
+                const int c = c0 + k;
+                const float w = __shfl_sync(0xffffffffu, c < 32 ? mine[0] : mine[1], c & 31);
+                if (!has || c >= chunks) continue;
+                acc[g][0] = fmaf(w, x[k].x, acc[g][0]);
+                acc[g][1] = fmaf(w, x[k].y, acc[g][1]);
+                acc[g][2] = fmaf(w, x[k].z, acc[g][2]);
+                acc[g][3] = fmaf(w, x[k].w, acc[g][3]);
+            }
         }
     }
 #pragma unroll
@@ -340,9 +352,21 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, const 
 }
 
 int launch_join(const AttnArgs &a, const Parts &parts) {
-    const unsigned grid = static_cast<unsigned>((a.total_tokens * a.H + 7) / 8);
-    if (a.dtype == RHZ_DTYPE_BF16) attn_join_kernel<__nv_bfloat16><<<grid, 256, 0, a.stream>>>(a, parts);
-    else attn_join_kernel<float><<<grid, 256, 0, a.stream>>>(a, parts);
+    // Its launch overlaps the end of the kernel before it.
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((a.total_tokens * a.H + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = a.stream;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    const bool few = parts.most <= 8, bf16 = a.dtype == RHZ_DTYPE_BF16;
+    auto *kernel = bf16 ? (few ? attn_join_kernel<__nv_bfloat16, 4> : attn_join_kernel<__nv_bfloat16, 16>)
+                        : (few ? attn_join_kernel<float, 4> : attn_join_kernel<float, 16>);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, parts);
+    if (e != cudaSuccess) return set_error(RHZ_ERR_DEVICE, "attn_join_kernel: %s", cudaGetErrorString(e));
     return check_launch("attn_join_kernel");
 }
 

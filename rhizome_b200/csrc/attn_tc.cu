@@ -673,17 +673,25 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 ++qn;
                 const int rows = g.rows, pages = KEYS / rows;
+                int ids = -1, page0 = 0;
                 for (int j = 0; j < tiles && ok; ++j) {
                     const int key = u.kbeg + j * KEYS;
                     int at = 0;          // this lane's page: its first row in the cache
                     bool there = false;
                     uint32_t valid = 1;
                     if (PAGED) {
+                        // The table's entries of 32 pages at a time, a lane each: one
+                        // load per tile would keep each tile back by its latency.
+                        const int last = (min(key + KEYS, u.keys) - 1) >> a.shift;
+                        if (j == 0 || last >= page0 + 32) {
+                            page0 = key >> a.shift;
+                            ids = page0 + lane < a.width ? a.block_table[u.seq * a.width + page0 + lane] : -1;
+                        }
                         const int mine = key + lane * rows;
+                        const int block = __shfl_sync(0xffffffffu, ids, min(max((mine >> a.shift) - page0, 0), 31));
                         if (lane < pages && mine < u.keys) {
-                            const int64_t block = a.block_table[u.seq * a.width + (mine >> a.shift)];
                             there = block >= 0 && block < a.num_blocks;
-                            at = static_cast<int>(((block * a.Hkv + u.kvh) << a.shift) + (mine & ((1 << a.shift) - 1)));
+                            at = static_cast<int>(((static_cast<int64_t>(block) * a.Hkv + u.kvh) << a.shift) + (mine & ((1 << a.shift) - 1)));
                         }
                         valid = __ballot_sync(0xffffffffu, there);
                     }

@@ -275,14 +275,23 @@ __global__ void __launch_bounds__(WARPS * 32)
 // The recurrence over a tree of drafted tokens: node t of sequence i starts
 // from the state of its parent node, S_t = step(S_parent(t)), or from the
 // pool's slot where the parent is -1, and every node's state is written out.
-// The rows of S never mix, so a warp that owns RPW rows walks the whole tree
+// The rows of S never mix, so a warp that owns 4 NR rows walks the whole tree
 // by itself: a node whose parent is the node before it finds the parent's
 // rows in registers, any other reads back what this warp wrote for the parent
-// (the same lanes at the same addresses, so program order is enough). The
-// traffic that cannot be avoided is the d x d f32 state written per node and
-// head; k, q, v and the gates of the next node are loaded while the current
-// one is computed, so the serial chain is two row products and an update.
-template <typename T, int RPW, int NV, int WARPS>
+// (the same lanes at the same addresses, so program order is enough).
+//
+// The traffic that cannot be avoided is the d x d f32 state written per node
+// and head. Eight lanes share a row here (lane 8 g + c: rows g + 4 i, columns
+// 4 c + 32 j): a row's product is 4 NJ multiply-adds and three shuffles, and
+// its sum is where it is needed, on the eight lanes that update the row. (A
+// whole warp to a row, as in the kernels above, took twice as many
+// instructions and was bound by them: 840 us for 32 trees of up to 64 nodes,
+// 32 heads, against 404 us of traffic.) The tree's q, k, v, gates and parents
+// come into shared memory first, all at once: fetched one node ahead they still
+// kept every node waiting for memory (650 us). Only a parent's rows are
+// fetched node by node, one ahead, unless the parent is the node before.
+// EXACT: d == 32 NJ, no bounds checks on columns and rows.
+template <typename T, int NR, int NJ, int WARPS, bool EXACT>
 __global__ void __launch_bounds__(WARPS * 32)
     gdr_tree_kernel(T *__restrict__ o, float *states, const float *__restrict__ pool,
                     const int32_t *__restrict__ slots, const int32_t *__restrict__ cu,
@@ -294,96 +303,178 @@ __global__ void __launch_bounds__(WARPS * 32)
     const int64_t seq = item / H;
     const int h = static_cast<int>(item - seq * H);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row0 = blockIdx.y * (WARPS * RPW) + warp * RPW;
-    if (row0 >= d) return;
-    constexpr int SHIFT = 5 - Log2<RPW>::value;
-    const int myrow = row0 + (lane >> SHIFT);
-    const bool writer = (lane & ((1 << SHIFT) - 1)) == 0 && myrow < d;
-    const int64_t dd = static_cast<int64_t>(d) * d;
+    const int row0 = (blockIdx.y * WARPS + warp) * (4 * NR) + (lane >> 3);  // and every fourth from there
+    const int col0 = 4 * (lane & 7);
+    const bool writer = (lane & 7) == 0;
+    const int dd = d * d;
     const int64_t first = min(max(static_cast<int64_t>(cu[seq]), int64_t{0}), total);
     const int64_t last = min(max(static_cast<int64_t>(cu[seq + 1]), first), total);
     const int m = static_cast<int>(min(last - first, static_cast<int64_t>(INT32_MAX)));
     const int64_t slot = !pool ? 0 : slots ? static_cast<int64_t>(slots[seq]) : seq;
     const bool valid = !pool || (slot >= 0 && slot < num_slots);
     const float *root = pool && valid ? pool + (slot * H + h) * dd : nullptr;
-    const int64_t row_stride = static_cast<int64_t>(H) * d;
+    const int nodes = min(m, most);
+    T *o0 = o + (first * H + h) * d;
+    float *s0 = states + (first * H + h) * dd;
+    const int64_t node_state = static_cast<int64_t>(H) * dd;
+    const int node_row = H * d;
 
-    float s[RPW][NV][4];
-    auto fetch = [&](const float *S) {  // this warp's rows of a state, zeros without one
+    // q, k, v [nodes][d], alpha, beta, parent [nodes].
+    extern __shared__ float4 tree_smem[];
+    T *sq = reinterpret_cast<T *>(tree_smem), *sk = sq + most * d, *sv = sk + most * d;
+    float *sa = reinterpret_cast<float *>(sv + most * d + (most * d & 1)), *sb = sa + most;
+    int *sp = reinterpret_cast<int *>(sb + most);
+    {
+        const int64_t at0 = (first * H + h) * d;
+        if (EXACT) {
+            constexpr int PER = 16 / sizeof(T), PIECES = 32 * NJ / PER;
+            for (int e = threadIdx.x; e < nodes * PIECES; e += WARPS * 32) {
+                const int t = e / PIECES, c = (e - t * PIECES) * PER;
+                const int64_t from = at0 + static_cast<int64_t>(t) * node_row + c;
+                *reinterpret_cast<uint4 *>(sq + t * d + c) = *reinterpret_cast<const uint4 *>(q + from);
+                *reinterpret_cast<uint4 *>(sk + t * d + c) = *reinterpret_cast<const uint4 *>(k + from);
+                *reinterpret_cast<uint4 *>(sv + t * d + c) = *reinterpret_cast<const uint4 *>(v + from);
+            }
+        } else {
+            for (int e = threadIdx.x; e < nodes * d; e += WARPS * 32) {
+                const int t = e / d;
+                const int64_t from = at0 + static_cast<int64_t>(t) * node_row + (e - t * d);
+                sq[e] = q[from];
+                sk[e] = k[from];
+                sv[e] = v[from];
+            }
+        }
+        for (int t = threadIdx.x; t < nodes; t += WARPS * 32) {
+            sa[t] = alpha[(first + t) * H + h];
+            sb[t] = beta[(first + t) * H + h];
+            sp[t] = parent ? parent[first + t] : t - 1;
+        }
+    }
+    __syncthreads();
+
+    float s[NR][NJ][4], ahead[NR][NJ][4];
+    auto fetch = [&](const float *S, float (&to)[NR][NJ][4]) {  // this lane's part of a state, zeros without one
 #pragma unroll
-        for (int r = 0; r < RPW; ++r)
+        for (int i = 0; i < NR; ++i)
 #pragma unroll
-            for (int c = 0; c < NV; ++c) {
-                const int j = 128 * c + 4 * lane;
-                if (S != nullptr && row0 + r < d) {
-                    load4(S + static_cast<int64_t>(row0 + r) * d + j, vec, nvalid(d, j), s[r][c]);
+            for (int j = 0; j < NJ; ++j) {
+                const int row = row0 + 4 * i, col = col0 + 32 * j;
+                if (EXACT && S != nullptr) {
+                    const float4 x = *reinterpret_cast<const float4 *>(S + row * d + col);
+                    to[i][j][0] = x.x; to[i][j][1] = x.y; to[i][j][2] = x.z; to[i][j][3] = x.w;
+                } else if (S != nullptr && row < d) {
+                    load4(S + row * d + col, vec, nvalid(d, col), to[i][j]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[r][c][e] = 0.f;
+                    for (int e = 0; e < 4; ++e) to[i][j][e] = 0.f;
                 }
             }
     };
-    float kk[NV][4], qq[NV][4], kn[NV][4], qn[NV][4], vn, an, bn;
-    int pn;
-    auto node = [&](int t) {  // the next node's inputs
-        const int64_t tok = first + t;
-        const int64_t at = tok * row_stride + static_cast<int64_t>(h) * d;
+    // Sums over a row's columns of s[i][.] x[.], on all eight lanes of the row.
+    auto dots = [&](const float (&x)[NJ][4], float (&sum)[NR]) {
 #pragma unroll
-        for (int c = 0; c < NV; ++c) {
-            const int j = 128 * c + 4 * lane;
-            load4(k + at + j, vec, nvalid(d, j), kn[c]);
-            load4(q + at + j, vec, nvalid(d, j), qn[c]);
+        for (int i = 0; i < NR; ++i) {
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[e] = fmaf(s[i][j][e], x[j][e], part[e]);
+            sum[i] = (part[0] + part[1]) + (part[2] + part[3]);
         }
-        vn = myrow < d ? to_f32(v[at + myrow]) : 0.f;
-        an = alpha[tok * H + h];
-        bn = beta[tok * H + h];
-        pn = parent ? parent[tok] : t - 1;
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1)
+#pragma unroll
+            for (int i = 0; i < NR; ++i) sum[i] += __shfl_xor_sync(FULL, sum[i], off);
+    };
+    struct alignas(4 * sizeof(T)) Four { T x[4]; };
+    auto columns = [&](const T *row, float (&x)[NJ][4]) {  // this lane's columns of a row in shared memory
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            if (EXACT) {
+                const Four f = *reinterpret_cast<const Four *>(row + col0 + 32 * j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[j][e] = to_f32(f.x[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[j][e] = col0 + 32 * j + e < d ? to_f32(row[col0 + 32 * j + e]) : 0.f;
+            }
+        }
     };
     uint64_t live = 0;  // nodes that take part: their parent is -1 or a live node before them
-    int held = -2;      // the node whose state the registers hold (-1: the root's)
-    const int nodes = min(m, most);
-    if (nodes > 0) node(0);
+    auto begin = [&](int t) -> int {  // notes whether node t takes part; its parent
+        const int p = sp[t];
+        if (p == -1 || (p >= 0 && p < t && (live >> p & 1))) live |= uint64_t{1} << t;
+        return p;
+    };
+    int held = -2;   // the node whose state s holds
+    int ready = -2;  // the node whose state `ahead` holds (-1: the root's)
+    int pn = nodes > 0 ? begin(0) : -2;
+    if (live & 1) {
+        fetch(root, ahead);
+        ready = -1;
+    }
     for (int t = 0; t < nodes; ++t) {
         const int p = pn;
-        const float a = an, b = bn, vm = vn;
+        const bool takes_part = live >> t & 1;
+        if (takes_part && p != held) {
+            if (p != ready) fetch(p < 0 ? root : s0 + p * node_state, ahead);
+            ready = -2;
 #pragma unroll
-        for (int c = 0; c < NV; ++c)
+            for (int i = 0; i < NR; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                kk[c][e] = kn[c][e];
-                qq[c][e] = qn[c][e];
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i][j][e] = ahead[i][j][e];
+        }
+        if (t + 1 < nodes) {
+            pn = begin(t + 1);
+            // A parent before t: its rows are written (by this warp) already.
+            if ((live >> (t + 1) & 1) && pn != t) {
+                fetch(pn < 0 ? root : s0 + pn * node_state, ahead);
+                ready = pn;
             }
-        if (t + 1 < nodes) node(t + 1);
-        const int64_t tok = first + t;
-        T *op = o + tok * row_stride + static_cast<int64_t>(h) * d;
-        if (p < -1 || p >= t || (p >= 0 && !(live >> p & 1))) {
-            if (writer) op[myrow] = from_f32<T>(0.f);
+        }
+        T *op = o0 + static_cast<int64_t>(t) * node_row;
+        if (!takes_part) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                if (writer && (EXACT || row0 + 4 * i < d)) op[row0 + 4 * i] = from_f32<T>(0.f);
             continue;
         }
-        live |= uint64_t{1} << t;
-        if (p != held) fetch(p < 0 ? root : states + ((first + p) * H + h) * dd);
         held = t;
-        float vr[RPW], sk[RPW], ov[RPW], mine;
+        const float a = sa[t], b = sb[t];
+        float sum[NR], kk[NJ][4];
+        columns(sk + t * d, kk);
+        dots(kk, sum);
+        float *St = s0 + t * node_state;
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) vr[r] = __shfl_sync(FULL, vm, r << SHIFT);
-        row_dots<RPW, NV>(s, kk, lane, sk, mine);
-        rank1_update<RPW, NV>(s, kk, sk, vr, a, b);
-        float *St = states + (tok * H + h) * dd;
+        for (int i = 0; i < NR; ++i) {
+            const float vi = EXACT || row0 + 4 * i < d ? to_f32(sv[t * d + row0 + 4 * i]) : 0.f;
+            const float bsk = b * sum[i], bv = b * vi;
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            if (row0 + r < d) {
+            for (int j = 0; j < NJ; ++j) {
 #pragma unroll
-                for (int c = 0; c < NV; ++c) {
-                    const int j = 128 * c + 4 * lane;
-                    store4(St + static_cast<int64_t>(row0 + r) * d + j, vec, nvalid(d, j), s[r][c]);
+                for (int e = 0; e < 4; ++e) {
+                    const float decayed = a * (s[i][j][e] - bsk * kk[j][e]);
+                    s[i][j][e] = decayed + bv * kk[j][e];
                 }
+                const int row = row0 + 4 * i, col = col0 + 32 * j;
+                if (EXACT)
+                    *reinterpret_cast<float4 *>(St + row * d + col) = make_float4(s[i][j][0], s[i][j][1], s[i][j][2], s[i][j][3]);
+                else if (row < d)
+                    store4(St + row * d + col, vec, nvalid(d, col), s[i][j]);
             }
         }
-        row_dots<RPW, NV>(s, qq, lane, ov, mine);
-        if (writer) op[myrow] = valid ? from_f32<T>(mine) : from_f32<T>(nanf(""));
+        columns(sq + t * d, kk);
+        dots(kk, sum);
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (writer && (EXACT || row0 + 4 * i < d)) op[row0 + 4 * i] = valid ? from_f32<T>(sum[i]) : from_f32<T>(nanf(""));
     }
-    for (int64_t t = nodes; t < m; ++t) {  // past the bound: not part of the tree
-        if (writer) o[(first + t) * row_stride + static_cast<int64_t>(h) * d + myrow] = from_f32<T>(0.f);
+    for (int t = nodes; t < m; ++t) {  // past the bound: not part of the tree
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (writer && (EXACT || row0 + 4 * i < d)) o0[static_cast<int64_t>(t) * node_row + row0 + 4 * i] = from_f32<T>(0.f);
     }
 }
 
@@ -593,27 +684,34 @@ int launch_multistep_t(const MultistepArgs &a) {
     return check_launch("gdr_multistep_kernel");
 }
 
-template <typename T, int RPW, int NV, int WARPS>
+template <typename T, int NR, int NJ, int WARPS>
 int launch_tree_t(const TreeArgs &a) {
-    dim3 grid(static_cast<unsigned>(a.n * a.H), (a.d + WARPS * RPW - 1) / (WARPS * RPW));
+    dim3 grid(static_cast<unsigned>(a.n * a.H), (a.d + WARPS * 4 * NR - 1) / (WARPS * 4 * NR));
     const bool vec = (a.d % 4) == 0;
-    gdr_tree_kernel<T, RPW, NV, WARPS><<<grid, WARPS * 32, 0, a.stream>>>(
+    auto *kernel = a.d == 32 * NJ ? gdr_tree_kernel<T, NR, NJ, WARPS, true> : gdr_tree_kernel<T, NR, NJ, WARPS, false>;
+    const size_t smem = static_cast<size_t>(a.most) * (3 * a.d * sizeof(T) + 3 * 4) + 16;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return set_error(RHZ_ERR_DEVICE, "gdr_tree_kernel: %s", cudaGetErrorString(e));
+    kernel<<<grid, WARPS * 32, smem, a.stream>>>(
         static_cast<T *>(a.o), a.states, a.pool, a.slots, a.cu_seqlens, a.parent,
         static_cast<const T *>(a.q), static_cast<const T *>(a.k), static_cast<const T *>(a.v),
         a.alpha, a.beta, a.total_tokens, a.most, a.num_slots, a.H, a.d, vec);
     return check_launch("gdr_tree_kernel");
 }
 
+template <typename T>
+int launch_tree_d(const TreeArgs &a) {
+    if (a.d <= 32) return launch_tree_t<T, 2, 1, 4>(a);
+    if (a.d <= 64) return launch_tree_t<T, 2, 2, 8>(a);
+    if (a.d <= 128) return launch_tree_t<T, 2, 4, 8>(a);
+    return launch_tree_t<T, 1, 8, 8>(a);
+}
+
 }  // namespace
 
 int launch_tree(const TreeArgs &a) {
     if (a.n == 0 || a.total_tokens == 0) return RHZ_OK;
-    if (a.dtype == RHZ_DTYPE_BF16) {
-        if (a.d <= 128) return launch_tree_t<__nv_bfloat16, 8, 1, 8>(a);
-        return launch_tree_t<__nv_bfloat16, 4, 2, 8>(a);
-    }
-    if (a.d <= 128) return launch_tree_t<float, 8, 1, 8>(a);
-    return launch_tree_t<float, 4, 2, 8>(a);
+    return a.dtype == RHZ_DTYPE_BF16 ? launch_tree_d<__nv_bfloat16>(a) : launch_tree_d<float>(a);
 }
 
 int launch_multistep(const MultistepArgs &a) {
