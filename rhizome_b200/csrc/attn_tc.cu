@@ -334,8 +334,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int e = 0; e < n; ++e, ++sn) {
                 const int h = e & 1, key = kbeg + e * HALF;
                 bool edge = e >= whole;
+                if (!loaded) {
+                    ok = wait(bars + 8 * (S_FULL + 2 * x + h), sp >> h & 1, abort);
+                    if (!ok) break;
+                    load(h);
+                }
                 uint32_t there[2] = {~0u, ~0u};
                 if (PAGED || edge) {
+                    // Not before the scores are there: only then is V's place in the ring
+                    // at most one lap from its turn, and the parity tells. (A warpgroup
+                    // without steps in a unit runs ahead of the ring.)
                     const uint32_t vt = it + (e | 1);  // this tile's V in the ring
                     const int vs = vt % C::STAGES;
                     ok = wait(bars + 8 * (KV_FULL + vs), (vt / C::STAGES) & 1, abort);
@@ -349,12 +357,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                     if (edge) clean_values<D, PAGED>(base + C::OFF_KV + vs * C::TILE, masks + 16 * vs, h, key, u.keys, full, r, spoiled + 16 * x + 4 * (i & 3), i + 1);
                 }
-                if (!loaded) {
-                    ok = wait(bars + 8 * (S_FULL + 2 * x + h), sp >> h & 1, abort);
-                    if (!ok) break;
-                    load(h);
-                    tmem_wait_ld();
-                }
+                tmem_wait_ld();
                 sp ^= 1u << h;
                 loaded = false;
                 const float2 c2 = make_float2(g.c2, g.c2);

@@ -294,6 +294,22 @@ def test_many_sequences():
     check_prompt([r.randrange(9) for _ in range(n)], 2, 1, 32, F32, seed=1)
 
 
+@pytest.mark.parametrize("d,nodes,H", [(128, 24, 8), (128, 64, 8), (64, 40, 16), (128, 2, 16), (128, 20, 32)])
+def test_many_trees_over_real_caches(d, nodes, H):
+    """More units than CTAs, most with rows for one of a CTA's two row tiles:
+    the idle half must not run ahead of the key ring."""
+    r = random.Random(nodes)
+    n = 60
+    check_tree([r.randint(0, 5000) for _ in range(n)], [r.randint(1, nodes) for _ in range(n)], H, 2 if H < 32 else 8, d, BF,
+               seed=nodes)
+
+
+def test_many_prompts_of_mixed_lengths():
+    r = random.Random(8)
+    check_prompt([r.choice([1, 30, 100, 128, 200, 700]) for _ in range(60)], 16, 4, 128, BF, seed=8)
+    check_prompt([r.choice([1, 30, 100, 128, 200, 700]) for _ in range(60)], 8, 8, 64, BF, seed=9)
+
+
 # ------------------------------------------------------------------ a step as an engine runs it
 
 @pytest.mark.parametrize("dtype", [BF, F32])
