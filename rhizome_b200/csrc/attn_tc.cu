@@ -38,11 +38,13 @@ using namespace attn;
 using namespace sm100;
 
 constexpr int ROWS = 128;   // query rows of a tile
-constexpr int KEYS = 128;   // keys of a tile
-constexpr int HALF = 64;    // keys of a step
+constexpr int KEYS = 64;    // keys of a step
 constexpr int THREADS = 384;
 constexpr int WARP_MMA = 8, WARP_TMA = 10, WARP_SCHED = 11;  // (two of the first)
 constexpr int GROUP = 256;  // sequences whose unit counts the scheduler holds at a time
+#ifndef BATCH
+#define BATCH 8
+#endif
 constexpr float FREE = 65536.f;  // probabilities may reach this against a maximum that was not looked for
 constexpr float LAZY = 8.f; // a row's maximum may grow by 2^LAZY before O is rescaled
 
@@ -55,25 +57,27 @@ struct Unit {
     int32_t seq, kvh;
     int32_t first, t0, m, live;  // query rows: first row, this unit's first token, tokens, those taking part
     int32_t cached, keys;        // keys before the sequence's own, and in all
-    int32_t kbeg, n0, n1;        // first key, half key tiles of either row tile
+    int32_t kbeg, n0, n1;        // first key, steps of either row tile
     int32_t chunk, chunks;
 };
 
 template <int D>
 struct Cfg {
-    static constexpr int HALVES = D / 64;
-    static constexpr int TILE = KEYS * D * 2;              // a K, V or Q tile in bytes
-    static constexpr int STAGES = D == 128 ? 4 : 8;        // K and V tiles in flight
+    static constexpr int HALVES = D / 64;                  // 64 channels: one 128-byte row
+    static constexpr int Q_TILE = ROWS * D * 2;
+    static constexpr int TILE = KEYS * D * 2;              // K or V of a step
+    static constexpr int STAGES = D == 128 ? 4 : 8;        // of either in flight
     static constexpr int OFF_Q = 0;
-    static constexpr int OFF_KV = 2 * TILE;
-    static constexpr int OFF_OUT = OFF_KV + STAGES * TILE; // 4 KB per softmax warp: output rows on their way out
+    static constexpr int OFF_K = 2 * Q_TILE;
+    static constexpr int OFF_V = OFF_K + STAGES * TILE;
+    static constexpr int OFF_OUT = OFF_V + STAGES * TILE;  // 4 KB per softmax warp: output rows on their way out
     static constexpr int OFF_BAR = OFF_OUT + 8 * 4096;     // barriers, units, scheduler's counts
-    static constexpr int OFF_UNIT = OFF_BAR + 320;
+    static constexpr int OFF_UNIT = OFF_BAR + 448;
     static constexpr int OFF_MASK = OFF_UNIT + 256;
     static constexpr int OFF_MISC = OFF_MASK + 128;
     static constexpr int OFF_COUNT = OFF_MISC + 64;
     static constexpr int BYTES = OFF_COUNT + GROUP * 4 + 1024;
-    static constexpr uint32_t ID_QK = idesc_bf16(ROWS, HALF, false, false);
+    static constexpr uint32_t ID_QK = idesc_bf16(ROWS, KEYS, false, false);
     static constexpr uint32_t ID_PV = idesc_bf16(ROWS, D, false, true);
 };
 
@@ -81,12 +85,12 @@ struct Cfg {
 // main loop touches is addressed by 32-bit addresses: as generic pointers the
 // loop's invariants alone would push its score registers out to memory.
 enum Bar : uint32_t {
-    KV_FULL = 0, KV_EMPTY = 8, Q_FULL = 16, Q_EMPTY = 17,
-    S_FULL = 18, P_FULL = 22,  // [row tile][half of the key tile]
-    PV_DONE = 26, O_FULL = 28, // [row tile]: a step's output product, a unit's last
-    U_FULL = 30, U_EMPTY = 34, DRAIN = 38, NUM_BARS = 39
+    K_FULL = 0, K_EMPTY = 8, V_FULL = 16, V_EMPTY = 24, Q_FULL = 32, Q_EMPTY = 33,
+    S_FULL = 34, P_FULL = 38,  // [row tile][parity of the step]
+    PV_DONE = 42, O_FULL = 44, // [row tile]: a step's output product, a unit's last
+    U_FULL = 46, U_EMPTY = 50, DRAIN = 54, NUM_BARS = 55
 };
-static_assert(NUM_BARS * 8 <= 320 && 4 * sizeof(Unit) <= 256, "shared-memory layout");
+static_assert(NUM_BARS * 8 <= 448 && 4 * sizeof(Unit) <= 256, "shared-memory layout");
 
 struct TcArgs {
     AttnArgs a;
@@ -198,11 +202,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // zero, and values that are not finite in rows from key `full` on are noted
 // at `spoiled`. (A probability of zero does not keep them out of a product.)
 template <int D, bool PAGED>
-__device__ __forceinline__ void clean_values(uint32_t tile, uint32_t mask, int h, int key, int keys, int full, int r,
+__device__ __forceinline__ void clean_values(uint32_t tile, uint32_t mask, int key, int keys, int full, int r,
                                              uint32_t spoiled, int mark) {
     const int kr = r >> 1;
-    const uint32_t vrow = tile + (h * HALF + kr) * 128 + (D == 128 ? (r & 1) * 16384 : 0);
-    const bool exists = key + kr < keys && (!PAGED || (lds(mask + 8 * h + 4 * (kr >> 5)) >> (kr & 31) & 1u));
+    const uint32_t vrow = tile + kr * 128 + (D == 128 ? (r & 1) * (KEYS * 128) : 0);
+    const bool exists = key + kr < keys && (!PAGED || (lds(mask + 4 * (kr >> 5)) >> (kr & 31) & 1u));
     if (!exists || key + kr >= full) {
         bool bad = false;
 #pragma unroll 1
@@ -236,7 +240,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t base = smem_u32(smem);
     const uint32_t bars = base + C::OFF_BAR, abort = base + C::OFF_MISC + 4;
     Unit *units = reinterpret_cast<Unit *>(smem + C::OFF_UNIT);
-    const uint32_t masks = base + C::OFF_MASK;  // 16 bytes per ring stage: keys with memory behind them
+    // Keys of a step with memory behind them, 8 bytes a step, 16 steps (K's copies,
+    // which write it, are at most six steps ahead of any softmax that reads).
+    const uint32_t masks = base + C::OFF_MASK;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
     // Unit i of tile x met values that are not finite where not every row sees
     // them: word [x][i & 3] is i + 1. (Unit i + 4 comes when every warp is done with i.)
@@ -247,8 +253,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; ++i) {
-            bar_init(bars + 8 * (KV_FULL + i), 1);
-            bar_init(bars + 8 * (KV_EMPTY + i), 2);
+            bar_init(bars + 8 * (K_FULL + i), 1);
+            bar_init(bars + 8 * (K_EMPTY + i), 2);
+            bar_init(bars + 8 * (V_FULL + i), 1);
+            bar_init(bars + 8 * (V_EMPTY + i), 2);
         }
         bar_init(bars + 8 * Q_FULL, 1);
         bar_init(bars + 8 * Q_EMPTY, 2);
@@ -297,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int x = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + 256 + x * 128;
-        uint32_t sn = 0, on = 0, it = 0;  // steps and units done (mod 2^32) of this row tile, ring position of the unit's first tile
+        uint32_t sn = 0, on = 0, it = 0;  // steps and units done (mod 2^32) of this row tile, steps before the unit
         uint32_t sp = 0;          // phases of S_FULL waited for, one bit per half
         const int row_token = r / g.group, row_head = r - row_token * g.group;
         for (int i = 0; wait(bars + 8 * (U_FULL + (i & 3)), (i >> 2) & 1, abort); ++i) {
@@ -323,16 +331,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             bool ok = true;
             const int n = x ? u.n1 : u.n0;
             // Halves that every live row sees whole.
-            const int whole = min(max(full - kbeg, 0) / HALF, n);
+            const int whole = min(max(full - kbeg, 0) / KEYS, n);
             bool loaded = false;  // v holds step e's scores
             float v[2][32];
             auto load = [&](int h) {
                 tc_fence_after();
 #pragma unroll
-                for (int w = 0; w < 2; ++w) tmem_ld32(ts + HALF * h + 32 * w, v[w]);
+                for (int w = 0; w < 2; ++w) tmem_ld32(ts + KEYS * h + 32 * w, v[w]);
             };
             for (int e = 0; e < n; ++e, ++sn) {
-                const int h = e & 1, key = kbeg + e * HALF;
+                const int h = e & 1, key = kbeg + e * KEYS;
                 bool edge = e >= whole;
                 if (!loaded) {
                     ok = wait(bars + 8 * (S_FULL + 2 * x + h), sp >> h & 1, abort);
@@ -340,22 +348,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                     load(h);
                 }
                 uint32_t there[2] = {~0u, ~0u};
-                if (PAGED || edge) {
+                const uint32_t nth = it + e;
+                if (PAGED) {
+                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                                 : "=r"(there[0]), "=r"(there[1])
+                                 : "r"(masks + 8 * (nth & 15))
+                                 : "memory");
+                    edge |= (there[0] & there[1]) != ~0u;
+                }
+                if (edge) {
                     // Not before the scores are there: only then is V's place in the ring
                     // at most one lap from its turn, and the parity tells. (A warpgroup
                     // without steps in a unit runs ahead of the ring.)
-                    const uint32_t vt = it + (e | 1);  // this tile's V in the ring
-                    const int vs = vt % C::STAGES;
-                    ok = wait(bars + 8 * (KV_FULL + vs), (vt / C::STAGES) & 1, abort);
+                    const int vs = nth % C::STAGES;
+                    ok = wait(bars + 8 * (V_FULL + vs), (nth / C::STAGES) & 1, abort);
                     if (!ok) break;
-                    if (PAGED) {
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            there[w] = lds(masks + 16 * vs + 8 * h + 4 * w);
-                            edge |= there[w] != ~0u;
-                        }
-                    }
-                    if (edge) clean_values<D, PAGED>(base + C::OFF_KV + vs * C::TILE, masks + 16 * vs, h, key, u.keys, full, r, spoiled + 16 * x + 4 * (i & 3), i + 1);
+                    clean_values<D, PAGED>(base + C::OFF_V + vs * C::TILE, masks + 8 * (nth & 15), key, u.keys, full, r, spoiled + 16 * x + 4 * (i & 3), i + 1);
                 }
                 tmem_wait_ld();
                 sp ^= 1u << h;
@@ -369,20 +377,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const float2 f2 = make_float2(from, from);
                     part[0] = part[1] = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int b = 0; b < 32; b += 8) {
-                        float2 y[8];
+                    for (int b = 0; b < 32; b += BATCH) {
+                        float2 y[BATCH];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
+                        for (int k = 0; k < BATCH; ++k) {
                             const int c = 2 * (b + k);
                             y[k] = fma2(make_float2(v[c / 32][c % 32], v[c / 32][c % 32 + 1]), c2, f2);
                         }
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
+                        for (int k = 0; k < BATCH; ++k) {
                             y[k].x = ex2(y[k].x);
                             y[k].y = ex2(y[k].y);
                         }
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
+                        for (int k = 0; k < BATCH; ++k) {
                             part[k & 1] = add2(part[k & 1], y[k]);
                             p[b + k] = pack_bf16(y[k].x, y[k].y);
                         }
@@ -442,7 +450,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                     exponentials();
                 }
-                tmem_st32u(ts + HALF * h, p);
+                tmem_st32u(ts + KEYS * h, p);
                 // The next step's scores come while the probabilities go, if they are there already.
                 if (e + 1 < n && __all_sync(0xffffffffu, bar_test(bars + 8 * (S_FULL + 2 * x + (h ^ 1)), sp >> (h ^ 1) & 1))) {
                     load(h ^ 1);
@@ -456,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (loaded) tmem_wait_ld();
             }
             if (!ok) break;
-            it += 2 * ((max(u.n0, u.n1) + 1) / 2);
+            it += max(u.n0, u.n1);
             bool bad = false;
             if (n > 0) {
                 if (!wait(bars + 8 * (O_FULL + x), on & 1, abort)) break;
@@ -469,7 +477,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int head = u.kvh * g.group + row_head;
             const bool split = PAGED && u.chunks > 1;
             if (bad) {
-                const int kend = min(u.keys, u.kbeg + n * HALF);
+                const int kend = min(u.keys, u.kbeg + n * KEYS);
                 for (int w = 0; w < 32; ++w) {  // the warp takes its own 32 rows
                     const int rr = (warp & 3) * 32 + w;
                     const Sight theirs{__shfl_sync(0xffffffffu, all, w), __shfl_sync(0xffffffffu, bits, w)};
@@ -546,7 +554,42 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        // Copies of K or V: the steps' pages are found and issued here by two
+        // warps, one each (a box takes its issuing warp some 60 cycles, and a
+        // step has 16 of them where a page is 16 positions; one warp for both
+        // needed 1,700 cycles a step). Lane l copies half l % HALVES of page l / HALVES.
+        const int rows = g.rows, pages = KEYS / rows;
+        int ids = -1, page0 = 0;  // the table's entries of 32 pages at a time, a lane each
+        int place = 0;            // the first row of this lane's page in the cache
+        uint32_t there = 0;       // lanes whose page has memory behind it
+        auto find_pages = [&](const Unit &u, int j) {
+            const int key = u.kbeg + j * KEYS;
+            const int last = (min(key + KEYS, u.keys) - 1) >> a.shift;
+            if (j == 0 || last >= page0 + 32) {
+                page0 = key >> a.shift;
+                ids = page0 + lane < a.width ? a.block_table[u.seq * a.width + page0 + lane] : -1;
+            }
+            const int mine = key + lane / C::HALVES * rows;
+            const int block = __shfl_sync(0xffffffffu, ids, min(max((mine >> a.shift) - page0, 0), 31));
+            const bool has = lane < pages * C::HALVES && mine < u.keys && block >= 0 && block < a.num_blocks;
+            there = __ballot_sync(0xffffffffu, has);
+            place = static_cast<int>(((static_cast<int64_t>(block) * a.Hkv + u.kvh) << a.shift) + (mine & ((1 << a.shift) - 1)));
+        };
+        auto copy_step = [&](const Unit &u, int j, uint32_t full, uint32_t dst, const CUtensorMap *tm) {
+            if (PAGED) {
+                if (lane == 0) bar_expect(full, __popc(there) * rows * 128);
+                __syncwarp();
+                if (there >> lane & 1u)
+                    load_2d(dst + lane % C::HALVES * (KEYS * 128) + lane / C::HALVES * rows * 128, tm, lane % C::HALVES * 64, place, full);
+            } else {
+                if (lane == 0) bar_expect(full, C::TILE);
+                __syncwarp();
+                if (lane < C::HALVES) load_3d(dst + lane * (KEYS * 128), tm, lane * 64, u.kvh, u.first + u.kbeg + j * KEYS, full);
+            }
+            __syncwarp();
+        };
         if (warp == WARP_SCHED) {
+            // Resolves units, and copies V.
             // Units in order of falling cost: unit l of a sequence is its row block
             // l / chunks (later blocks see more keys), and all sequences' units
             // of one l come together, the highest l first; dealt to the CTAs in
@@ -562,9 +605,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int i = lane; i < GROUP; i += 32) n += __popc(__ballot_sync(0xffffffffu, counts[i] > l));
                 return n;
             };
-            bool going = true;
-#pragma unroll 1
-            for (int i = 0; going; ++i) {
+            // Unit i of this CTA, passed on to the other roles.
+            bool ok = true;
+            auto resolve = [&](int i) -> Unit {
+                bool going = true;
                 const int64_t x64 = static_cast<int64_t>(i) * G + ((i & 1) ? G - 1 - blockIdx.x : blockIdx.x);
                 const int x = static_cast<int>(min(x64, static_cast<int64_t>(INT32_MAX)));
                 const int want = x / a.Hkv;
@@ -645,25 +689,51 @@ __global__ void __launch_bounds__(THREADS, 1)
                         const int t = u.t0 + y * g.tok;
                         int end = t >= u.live ? 0 : stop;
                         if (!(PAGED && a.parent)) end = min(end, cached + t + g.tok);
-                        const int halves = max(end - u.kbeg + HALF - 1, 0) / HALF;
-                        (y ? u.n1 : u.n0) = halves;
+                        const int steps = max(end - u.kbeg + KEYS - 1, 0) / KEYS;
+                        (y ? u.n1 : u.n0) = steps;
                     }
                 }
-                if (i >= 4 && !wait(bars + 8 * (U_EMPTY + (i & 3)), ((i >> 2) - 1) & 1, abort)) break;
-                if (lane == 0) {
+                ok = ok && (i < 4 || wait(bars + 8 * (U_EMPTY + (i & 3)), ((i >> 2) - 1) & 1, abort));
+                if (ok && lane == 0) {
                     units[i & 3] = u;
                     bar_arrive(bars + 8 * (U_FULL + (i & 3)));
                 }
                 __syncwarp();
+                return u;
+            };
+            Unit u = resolve(0);
+            uint32_t vn = 0;  // tiles issued
+#pragma unroll 1
+            for (int i = 0; ok && u.valid; ++i) {
+                const int steps = max(u.n0, u.n1), early = max(min(steps, C::STAGES), 1);
+                Unit after;
+#pragma unroll 1
+                for (int j = 0; ok && j < max(steps, 1); ++j) {
+                    if (steps > 0) {
+                        if (PAGED) find_pages(u, j);
+                        const int st = vn % C::STAGES;
+                        ok = vn < C::STAGES || wait(bars + 8 * (V_EMPTY + st), (vn / C::STAGES - 1) & 1, abort);
+                        if (!ok) break;
+                        copy_step(u, j, bars + 8 * (V_FULL + st), base + C::OFF_V + st * C::TILE, &tm_v);
+                        ++vn;
+                    }
+                    if (j + 1 == early) after = resolve(i + 1);  // well before K's copies come to it
+                }
+                u = after;
             }
+            if (lds(abort))  // copies in flight land before the CTA leaves
+                for (uint32_t k = vn > C::STAGES ? vn - C::STAGES : 0; k < vn; ++k)
+                    drain_wait(bars + 8 * (V_FULL + k % C::STAGES), (k / C::STAGES) & 1);
         } else if (warp == WARP_TMA) {
-            // K and V tiles in the order K0 V0 K1 V1 ..: one ring for both.
+            // Copies Q, and K as far ahead as its ring allows. (K and V have a ring
+            // each: in one, a K whose place was free waited behind a V whose place was not.)
             Unit u;
-            uint32_t it = 0, qn = 0;  // tiles and Q loads issued
+            uint32_t qn = 0, kn = 0;  // Q loads and tiles issued
             bool ok = true;
+#pragma unroll 1
             for (int i = 0; ok && next_unit(i, u); ++i) {
-                const int tiles = (max(u.n0, u.n1) + 1) / 2;
-                if (tiles == 0) continue;
+                const int steps = max(u.n0, u.n1);
+                if (steps == 0) continue;
                 if (qn > 0) ok = wait(bars + 8 * Q_EMPTY, (qn - 1) & 1, abort);
                 if (!ok) break;
                 if (lane == 0) {
@@ -671,69 +741,32 @@ __global__ void __launch_bounds__(THREADS, 1)
                     bar_expect(bars + 8 * Q_FULL, bytes * ((u.n0 > 0) + (u.n1 > 0)));
                     for (int x = 0; x < 2; ++x)
                         for (int h = 0; (x ? u.n1 : u.n0) > 0 && h < C::HALVES; ++h)
-                            load_3d(base + C::OFF_Q + x * C::TILE + h * 16384, &tm_q, h * 64, u.kvh * g.group,
-                                        u.first + u.t0 + x * g.tok, bars + 8 * Q_FULL);
+                            load_3d(base + C::OFF_Q + x * C::Q_TILE + h * (ROWS * 128), &tm_q, h * 64, u.kvh * g.group,
+                                    u.first + u.t0 + x * g.tok, bars + 8 * Q_FULL);
                 }
                 ++qn;
-                const int rows = g.rows, pages = KEYS / rows;
-                int ids = -1, page0 = 0;
-                for (int j = 0; j < tiles && ok; ++j) {
-                    const int key = u.kbeg + j * KEYS;
-                    int at = 0;          // this lane's page: its first row in the cache
-                    bool there = false;
-                    uint32_t valid = 1;
-                    if (PAGED) {
-                        // The table's entries of 32 pages at a time, a lane each: one
-                        // load per tile would keep each tile back by its latency.
-                        const int last = (min(key + KEYS, u.keys) - 1) >> a.shift;
-                        if (j == 0 || last >= page0 + 32) {
-                            page0 = key >> a.shift;
-                            ids = page0 + lane < a.width ? a.block_table[u.seq * a.width + page0 + lane] : -1;
+#pragma unroll 1
+                for (int j = 0; j < steps; ++j) {
+                    if (PAGED) find_pages(u, j);
+                    const int st = kn % C::STAGES;
+                    ok = kn < C::STAGES || wait(bars + 8 * (K_EMPTY + st), (kn / C::STAGES - 1) & 1, abort);
+                    if (!ok) break;
+                    if (PAGED && lane < 2) {  // which of the step's keys have memory behind them
+                        uint32_t w = ~0u;
+                        if (__popc(there) != pages * C::HALVES) {
+                            w = 0;
+                            for (int b = 0; b < 32; ++b) w |= (there >> ((lane * 32 + b) / rows * C::HALVES) & 1u) << b;
                         }
-                        const int mine = key + lane * rows;
-                        const int block = __shfl_sync(0xffffffffu, ids, min(max((mine >> a.shift) - page0, 0), 31));
-                        if (lane < pages && mine < u.keys) {
-                            there = block >= 0 && block < a.num_blocks;
-                            at = static_cast<int>(((static_cast<int64_t>(block) * a.Hkv + u.kvh) << a.shift) + (mine & ((1 << a.shift) - 1)));
-                        }
-                        valid = __ballot_sync(0xffffffffu, there);
+                        sts(masks + 8 * (kn & 15) + 4 * lane, w);
                     }
-                    for (int kv = 0; kv < 2; ++kv, ++it) {
-                        const int st = it % C::STAGES;
-                        const uint32_t lap = it / C::STAGES;
-                        if (lap > 0 && !wait(bars + 8 * (KV_EMPTY + st), (lap - 1) & 1, abort)) {
-                            ok = false;
-                            break;
-                        }
-                        const uint32_t dst = base + C::OFF_KV + st * C::TILE;
-                        const CUtensorMap *tm = kv ? &tm_v : &tm_k;
-                        if (PAGED) {
-                            if (kv == 1 && lane < 4) {  // which of the tile's keys have memory behind them
-                                uint32_t w = ~0u;
-                                if (__popc(valid) != pages) {
-                                    w = 0;
-                                    for (int b = 0; b < 32; ++b) w |= (valid >> ((lane * 32 + b) / rows) & 1u) << b;
-                                }
-                                sts(masks + 16 * st + 4 * lane, w);
-                            }
-                            __syncwarp();
-                            if (lane == 0) bar_expect(bars + 8 * (KV_FULL + st), __popc(valid) * rows * D * 2);
-                            __syncwarp();
-                            if (there)
-                                for (int h = 0; h < C::HALVES; ++h)
-                                    load_2d(dst + h * 16384 + lane * rows * 128, tm, h * 64, at, bars + 8 * (KV_FULL + st));
-                        } else if (lane == 0) {
-                            bar_expect(bars + 8 * (KV_FULL + st), C::TILE);
-                            for (int h = 0; h < C::HALVES; ++h)
-                                load_3d(dst + h * 16384, tm, h * 64, u.kvh, u.first + key, bars + 8 * (KV_FULL + st));
-                        }
-                        __syncwarp();
-                    }
+                    __syncwarp();
+                    copy_step(u, j, bars + 8 * (K_FULL + st), base + C::OFF_K + st * C::TILE, &tm_k);
+                    ++kn;
                 }
             }
             if (lds(abort)) {  // copies in flight land before the CTA leaves
-                for (uint32_t k = it > C::STAGES ? it - C::STAGES : 0; k < it; ++k)
-                    drain_wait(bars + 8 * (KV_FULL + (k % C::STAGES)), (k / C::STAGES) & 1);
+                for (uint32_t k = kn > C::STAGES ? kn - C::STAGES : 0; k < kn; ++k)
+                    drain_wait(bars + 8 * (K_FULL + k % C::STAGES), (k / C::STAGES) & 1);
                 if (qn > 0) drain_wait(bars + 8 * Q_FULL, (qn - 1) & 1);
             }
         } else if (warp < WARP_TMA) {
@@ -745,30 +778,29 @@ __global__ void __launch_bounds__(THREADS, 1)
             const bool chosen = elect_one();
             // A descriptor's address field counts 16 bytes: steps are added to
             // its low word (addresses stay below 2^18, so nothing carries).
-            const uint64_t like = sdesc_sw128(0, 16, 1024), like_v = sdesc_sw128(0, 16384, 1024);
+            const uint64_t like = sdesc_sw128(0, 16, 1024), like_v = sdesc_sw128(0, KEYS * 128, 1024);
             const uint32_t hi = static_cast<uint32_t>(like >> 32), hi_v = static_cast<uint32_t>(like_v >> 32);
             const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
-            const uint32_t q_lo = static_cast<uint32_t>(like) + ((base + C::OFF_Q + x * C::TILE) >> 4);
-            const uint32_t k_lo = static_cast<uint32_t>(like) + ((base + C::OFF_KV) >> 4);
-            const uint32_t v_lo = static_cast<uint32_t>(like_v) + ((base + C::OFF_KV) >> 4);
+            const uint32_t q_lo = static_cast<uint32_t>(like) + ((base + C::OFF_Q + x * C::Q_TILE) >> 4);
+            const uint32_t k_lo = static_cast<uint32_t>(like) + ((base + C::OFF_K) >> 4);
+            const uint32_t v_lo = static_cast<uint32_t>(like_v) + ((base + C::OFF_V) >> 4);
             auto qk = [&](int h, int st) {
-                const uint32_t ka = k_lo + st * (C::TILE >> 4) + h * (HALF * 128 >> 4), d = t0 + x * 128 + h * HALF;
+                const uint32_t ka = k_lo + st * (C::TILE >> 4), d = t0 + x * 128 + h * KEYS;
                 if (chosen) {
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                        mma_ss(d, q_lo + off, ka + off, hi, C::ID_QK, k > 0);
-                    }
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_ss(d, q_lo + (((k >> 2) * (ROWS * 128) + (k & 3) * 32) >> 4), ka + (((k >> 2) * (KEYS * 128) + (k & 3) * 32) >> 4),
+                               hi, C::ID_QK, k > 0);
                     commit(bars + 8 * (S_FULL + 2 * x + h));
                 }
                 __syncwarp();
             };
             auto pv = [&](int h, int st, bool more) {
-                const uint32_t va = v_lo + st * (C::TILE >> 4) + h * (HALF * 128 >> 4);
-                const uint32_t p = t0 + x * 128 + h * HALF, d = t0 + 256 + x * 128;
+                const uint32_t va = v_lo + st * (C::TILE >> 4);
+                const uint32_t p = t0 + x * 128 + h * KEYS, d = t0 + 256 + x * 128;
                 if (chosen) {
 #pragma unroll
-                    for (int k = 0; k < HALF / 16; ++k) mma_ts(d, p + 8 * k, va + k * (2048 >> 4), hi_v, C::ID_PV, more || k > 0);
+                    for (int k = 0; k < KEYS / 16; ++k) mma_ts(d, p + 8 * k, va + k * (2048 >> 4), hi_v, C::ID_PV, more || k > 0);
                     commit(bars + 8 * (PV_DONE + x));
                 }
                 __syncwarp();
@@ -778,34 +810,33 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
             };
             Unit u;
-            uint32_t it = 0, qn = 0, pp = 0;  // pp: phases of P_FULL waited for, one bit per half
+            uint32_t qn = 0, pp = 0;     // pp: phases of P_FULL waited for, one bit per parity
+            int ks = 0, vs = 0;          // places of the rings
+            uint32_t kp = 0, vp = 0;     // and the parities of their laps
             bool ok = true;
+            auto next = [](int &st, uint32_t &lap) {
+                if (++st == C::STAGES) {
+                    st = 0;
+                    lap ^= 1;
+                }
+            };
 #pragma unroll 1
             for (int i = 0; ok && next_unit(i, u); ++i) {
-                const int tiles = __shfl_sync(0xffffffffu, (max(u.n0, u.n1) + 1) / 2, 0);
+                const int steps = __shfl_sync(0xffffffffu, max(u.n0, u.n1), 0);
                 const int n = __shfl_sync(0xffffffffu, x ? u.n1 : u.n0, 0);
-                if (tiles == 0) continue;
-                int st = it % C::STAGES;
-                uint32_t lap = it / C::STAGES;
-                ok = wait(bars + 8 * Q_FULL, qn & 1, abort) && wait(bars + 8 * (KV_FULL + st), lap & 1, abort);
+                if (steps == 0) continue;
+                ok = wait(bars + 8 * Q_FULL, qn & 1, abort);
                 if (!ok) break;
+                // Step e: P is there; its product, then the scores of step e + 2 in its
+                // place. (Steps -2 and -1 are the first two scores. Every place of the
+                // rings is waited for and released also where this row tile has no use
+                // for it: an arrival on EMPTY belongs to the lap whose FULL it follows.)
 #pragma unroll 1
-                for (int h = 0; h < min(n, 2); ++h) qk(h, st);
-                done(bars + 8 * (KV_EMPTY + st));
-                if (tiles == 1) done(bars + 8 * Q_EMPTY);
-#pragma unroll 1
-                for (int j = 0; j < tiles; ++j) {
-                    // V of this key tile, K of the next.
-                    const int vs = st + 1 == C::STAGES ? 0 : st + 1, ks = vs + 1 == C::STAGES ? 0 : vs + 1;
-                    const uint32_t vlap = lap + (vs < st), klap = vlap + (ks < vs);
-                    // (Also where this row tile has no use for them: an arrival on
-                    // KV_EMPTY belongs to the lap whose KV_FULL it follows.)
-                    ok = wait(bars + 8 * (KV_FULL + vs), vlap & 1, abort);
-                    if (!ok) break;
-                    bool have_k = false;
-#pragma unroll 1
-                    for (int h = 0; h < 2; ++h) {
-                        const int e = 2 * j + h;  // P of this half is there: its product, then the scores that take its place
+                for (int e = -2; e < steps; ++e) {
+                    const int h = e & 1;
+                    if (e >= 0) {
+                        ok = wait(bars + 8 * (V_FULL + vs), vp, abort);
+                        if (!ok) break;
                         if (e < n) {
                             ok = wait(bars + 8 * (P_FULL + 2 * x + h), pp >> h & 1, abort);
                             if (!ok) break;
@@ -814,23 +845,18 @@ __global__ void __launch_bounds__(THREADS, 1)
                             pv(h, vs, e > 0);
                             if (e + 1 == n) done(bars + 8 * (O_FULL + x));
                         }
-                        if (j + 1 < tiles && !have_k) {
-                            ok = wait(bars + 8 * (KV_FULL + ks), klap & 1, abort);
-                            if (!ok) break;
-                            have_k = true;
-                        }
+                        done(bars + 8 * (V_EMPTY + vs));
+                        next(vs, vp);
+                    }
+                    if (e + 2 < steps) {
+                        ok = wait(bars + 8 * (K_FULL + ks), kp, abort);
+                        if (!ok) break;
                         if (e + 2 < n) qk(h, ks);
+                        done(bars + 8 * (K_EMPTY + ks));
+                        next(ks, kp);
+                        if (e + 3 == steps) done(bars + 8 * Q_EMPTY);
                     }
-                    if (!ok) break;
-                    done(bars + 8 * (KV_EMPTY + vs));
-                    if (j + 1 < tiles) {
-                        done(bars + 8 * (KV_EMPTY + ks));
-                        if (j + 2 == tiles) done(bars + 8 * Q_EMPTY);
-                    }
-                    st = ks;
-                    lap = klap;
                 }
-                it += 2 * tiles;
                 ++qn;
             }
             if (lds(abort) && chosen) {  // products in flight finish before TMEM is freed
