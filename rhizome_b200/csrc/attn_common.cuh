@@ -29,14 +29,15 @@ constexpr int MAX_NODES = 64;  // drafted tokens of one sequence (one bit each)
 struct Split {
     int least;  // keys per chunk at least (a multiple of 128)
     int most;   // chunks per sequence at most
-    __host__ __device__ int64_t span(int64_t L) const {
-        int64_t c = (L + most - 1) / most;
-        c = (c + 127) / 128 * 128;
-        return c < least ? least : c;
+    // (Lengths fit 31 bits: the entry refuses wider tables.)
+    __host__ __device__ int span(int64_t L) const {
+        const uint32_t c = (static_cast<uint32_t>(L) + most - 1) / most;
+        const int up = static_cast<int>((c + 127) / 128 * 128);
+        return up < least ? least : up;
     }
-    __host__ __device__ int64_t chunks(int64_t L) const {
-        const int64_t c = span(L);
-        return L <= 0 ? 1 : (L + c - 1) / c;
+    __host__ __device__ int chunks(int64_t L) const {
+        const uint32_t c = span(L);
+        return L <= 0 ? 1 : static_cast<int>((static_cast<uint32_t>(L) + c - 1) / c);
     }
     // The most chunks that any length up to L can have.
     int64_t bound(int64_t L) const {
@@ -83,24 +84,26 @@ inline Parts parts_at(void *ws, int64_t tokens, int H, int d, int64_t chunks) {
 // One sequence as the kernels see it: offsets clamped to the buffers, so that
 // no cu_seqlens, length or table can lead outside them.
 struct Seq {
-    int64_t first;   // first query row
-    int64_t m;       // query rows
-    int64_t live;    // of which take part (m, at most `most`)
-    int64_t cached;  // keys before the sequence's own rows (0 packed)
-    int64_t keys;    // cached + live
+    int first;   // first query row
+    int m;       // query rows
+    int live;    // of which take part (m, at most `most`)
+    int cached;  // keys before the sequence's own rows (0 packed)
+    int keys;    // cached + live
 };
 
+// (The entries refuse token counts and tables beyond 31 bits.)
 __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int64_t i) {
+    const int total = static_cast<int>(a.total_tokens);
     Seq s;
-    s.first = min(max(static_cast<int64_t>(a.cu_seqlens[i]), int64_t{0}), a.total_tokens);
-    s.m = min(max(static_cast<int64_t>(a.cu_seqlens[i + 1]), s.first), a.total_tokens) - s.first;
+    s.first = min(max(a.cu_seqlens[i], 0), total);
+    s.m = min(max(a.cu_seqlens[i + 1], s.first), total) - s.first;
     s.cached = 0;
     s.live = s.m;
     if (a.paged) {
-        const int64_t room = a.width << a.shift;
-        s.live = min(s.m, a.most);
-        s.cached = min(max(static_cast<int64_t>(a.cached[i]), int64_t{0}), room);
-        s.live = min(s.live, room - s.cached);  // rows whose own key has no table entry take no part
+        const int room = static_cast<int>(a.width << a.shift);
+        s.cached = min(max(a.cached[i], 0), room);
+        // Rows whose own key has no table entry take no part either.
+        s.live = min(min(s.m, static_cast<int>(a.most)), room - s.cached);
     }
     s.keys = s.cached + s.live;
     return s;

@@ -2,14 +2,17 @@
 // token or a small drafted tree, bf16, head widths 64 and 128.
 //
 // What bounds it is reading K and V once: a (sequence, K/V head) pair has at
-// most 32 rows here, 32 multiply-adds to a byte, an eighth of what the tensor
+// most 16 rows here, 16 multiply-adds to a byte, a sixteenth of what the tensor
 // cores could take at HBM's rate. So the unit of work is one warp's: a chunk of
 // one pair's keys (Split in attn_common.cuh), read in tiles of 32 keys that
 // the warp's own ring of TMA copies brings in; no warp waits for another. The
 // products run as mma.sync m16n8k16 from that ring (rows as m, so that every
 // row of the group shares each K and V byte), the softmax stays in registers.
 // Four warps with 48 KB in flight each keep an SM's share of HBM busy (44 KB
-// would cover one microsecond of it).
+// would cover one microsecond of it). 512 sequences of U{1..8192} keys, one
+// token, 16 heads over 4, pages of 16: 1,350 us, 6.2 TB/s, 0.95 of a plain copy's
+// rate, and 26 us to join the chunks; 74 sequences of 8,192 keys and four tokens: 448 us,
+// 5.5 TB/s (rows of masked nodes and one round of units more for some SMs).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -88,9 +91,9 @@ __device__ __forceinline__ uint32_t piece_at(int key, int c) {
     return (c >> 3) * (KEYS * 128) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
 }
 
-// MT 16-row tiles. Fragments (PTX, g = lane / 4, t = lane % 4): a score or
+// Fragments (PTX, g = lane / 4, t = lane % 4): a score or
 // output tile n holds rows g and g + 8, columns 8 n + 2 t and the next.
-template <int D, int MT>
+template <int D>
 __global__ void __launch_bounds__(32 * WARPS, 1)
     attn_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                      const __grid_constant__ RowsArgs g) {
@@ -240,12 +243,12 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
         __syncwarp();
         top_up(k);  // (the copies stop where too many units lie ahead: some may have no keys)
         // Q as A fragments, the rows' sight.
-        uint32_t q[MT][D / 16][4];
-        int all[2 * MT];
-        uint64_t bits[2 * MT];
-        const int used = min(u.live, MT * 16 / g.group) * g.group;  // rows with a token that takes part
+        uint32_t q[D / 16][4];
+        int all[2];
+        uint64_t bits[2];
+        const int used = min(u.live, 16 / g.group) * g.group;  // rows with a token that takes part
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
+        for (int i = 0; i < 2; ++i) {
             const int r = gq + 8 * i, t = r / g.group, of = r - t * g.group;
             all[i] = 0;
             bits[i] = 0;
@@ -262,19 +265,17 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
                                        static_cast<int64_t>(u.kvh * g.group + of) * D + 2 * tq;
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
-                q[i >> 1][c][i & 1] = has ? *reinterpret_cast<const uint32_t *>(src + 16 * c) : 0u;
-                q[i >> 1][c][2 + (i & 1)] = has ? *reinterpret_cast<const uint32_t *>(src + 16 * c + 8) : 0u;
+                q[c][i & 1] = has ? *reinterpret_cast<const uint32_t *>(src + 16 * c) : 0u;
+                q[c][2 + (i & 1)] = has ? *reinterpret_cast<const uint32_t *>(src + 16 * c + 8) : 0u;
             }
         }
-        float acc[MT][D / 8][4], top[2 * MT], sum[2 * MT];
+        float acc[D / 8][4], top[2], sum[2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n)
+            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
+        for (int i = 0; i < 2; ++i) {
             top[i] = -INFINITY;
             sum[i] = 0.f;
         }
@@ -319,31 +320,26 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
                 __syncwarp();
             }
             // Scores: 4 tiles of 8 keys.
-            float x[MT][4][4];
+            float x[4][4];
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[i][n][e] = 0.f;
+                for (int e = 0; e < 4; ++e) x[n][e] = 0.f;
 #pragma unroll
             for (int c = 0; c < D / 16; ++c)
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     uint32_t b[4];
                     ldsm4(b, kt + piece_at(16 * n + (lane & 7) + ((lane >> 4) << 3), 2 * c + ((lane >> 3) & 1)));
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        mma(x[i][2 * n], q[i][c], b[0], b[1]);
-                        mma(x[i][2 * n + 1], q[i][c], b[2], b[3]);
-                    }
+                    mma(x[2 * n], q[c], b[0], b[1]);
+                    mma(x[2 * n + 1], q[c], b[2], b[3]);
                 }
             // Softmax.
-            uint32_t p[MT][2][4];
+            uint32_t p[2][4];
             bool moved = false;
-            float keep[2 * MT];
+            float keep[2];
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 float best = top[i];
                 uint32_t m = ~0u;
                 if (edge) m = seen_word(all[i], bits[i], key) & valid;
@@ -351,7 +347,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float &s = x[i >> 1][n][2 * (i & 1) + e];
+                        float &s = x[n][2 * i + e];
                         s *= g.c2;
                         if (edge && !(m >> (8 * n + 2 * tq + e) & 1u)) s = -INFINITY;
                         best = fmaxf(best, s);
@@ -367,7 +363,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float &s = x[i >> 1][n][2 * (i & 1) + e];
+                        float &s = x[n][2 * i + e];
                         s = ex2(s - from);
                         part += s;
                     }
@@ -375,32 +371,25 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
             }
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-                    for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][n][e] *= keep[2 * i + (e >> 1)];
+                    for (int e = 0; e < 4; ++e) acc[n][e] *= keep[e >> 1];
             }
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    p[i][n][0] = pack_bf16(x[i][2 * n][0], x[i][2 * n][1]);
-                    p[i][n][1] = pack_bf16(x[i][2 * n][2], x[i][2 * n][3]);
-                    p[i][n][2] = pack_bf16(x[i][2 * n + 1][0], x[i][2 * n + 1][1]);
-                    p[i][n][3] = pack_bf16(x[i][2 * n + 1][2], x[i][2 * n + 1][3]);
-                }
+            for (int n = 0; n < 2; ++n) {
+                p[n][0] = pack_bf16(x[2 * n][0], x[2 * n][1]);
+                p[n][1] = pack_bf16(x[2 * n][2], x[2 * n][3]);
+                p[n][2] = pack_bf16(x[2 * n + 1][0], x[2 * n + 1][1]);
+                p[n][3] = pack_bf16(x[2 * n + 1][2], x[2 * n + 1][3]);
+            }
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
                     uint32_t b[4];
                     ldsm4t(b, vt + piece_at(16 * n + (lane & 7) + (((lane >> 3) & 1) << 3), 2 * c + (lane >> 4)));
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        mma(acc[i][2 * c], p[i][n], b[0], b[1]);
-                        mma(acc[i][2 * c + 1], p[i][n], b[2], b[3]);
-                    }
+                    mma(acc[2 * c], p[n], b[0], b[1]);
+                    mma(acc[2 * c + 1], p[n], b[2], b[3]);
                 }
             __syncwarp();  // every lane has read the tile
             copy(k);
@@ -409,7 +398,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
         bad = __any_sync(0xffffffffu, bad);
         const bool split = u.chunks > 1;
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
+        for (int i = 0; i < 2; ++i) {
             float l = sum[i];
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -427,13 +416,13 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n)
                     dst[4 * n] = l == 0.f ? make_float2(0.f, 0.f)
-                                          : make_float2(acc[i >> 1][n][2 * (i & 1)] * inv, acc[i >> 1][n][2 * (i & 1) + 1] * inv);
+                                          : make_float2(acc[n][2 * i] * inv, acc[n][2 * i + 1] * inv);
             } else {
                 if (tq == 0 && a.lse) a.lse[token * a.H + head] = l2 * LN2;
                 uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(a.o) + (token * a.H + head) * D + 2 * tq);
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n)
-                    dst[4 * n] = l == 0.f ? 0u : pack_bf16(acc[i >> 1][n][2 * (i & 1)] * inv, acc[i >> 1][n][2 * (i & 1) + 1] * inv);
+                    dst[4 * n] = l == 0.f ? 0u : pack_bf16(acc[n][2 * i] * inv, acc[n][2 * i + 1] * inv);
             }
         }
         if (bad) {
@@ -468,7 +457,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
             }
 }
 
-template <int D, int MT>
+template <int D>
 int launch_t(const AttnArgs &a, const Parts &parts, Split split) {
     RowsArgs g{};
     g.a = a;
@@ -493,25 +482,23 @@ int launch_t(const AttnArgs &a, const Parts &parts, Split split) {
     if (units > INT32_MAX) return set_error(RHZ_ERR_SHAPE, "attention over %lld units exceeds int32 indexing", (long long)units);
     const int64_t ctas = (units + WARPS - 1) / WARPS;
     const unsigned grid = static_cast<unsigned>(ctas < sms ? ctas : sms);
-    cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::BYTES);
+    cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::BYTES);
     if (e != cudaSuccess) return set_error(RHZ_ERR_DEVICE, "attn_rows_kernel: %s", cudaGetErrorString(e));
-    attn_rows_kernel<D, MT><<<grid, 32 * WARPS, Cfg<D>::BYTES, a.stream>>>(tk, tv, g);
+    attn_rows_kernel<D><<<grid, 32 * WARPS, Cfg<D>::BYTES, a.stream>>>(tk, tv, g);
     return check_launch("attn_rows_kernel");
 }
 
 }  // namespace
 
-// Two 16-row tiles at most: beyond 32 rows the products outgrow what
-// mma.sync can do at HBM's rate, and the tcgen05 form takes over.
+// One 16-row tile: with two, 74 sequences of 8,192 keys and 32 rows took 1,088 us
+// here and 552 us as a row tile of the tcgen05 form.
 bool attn_rows_supports(const AttnArgs &a) {
     return a.paged && a.dtype == RHZ_DTYPE_BF16 && (a.d == 64 || a.d == 128) && a.n_seq <= MAX_SEQ &&
-           a.most * (a.H / a.Hkv) <= 32;
+           a.most * (a.H / a.Hkv) <= 16;
 }
 
 int launch_attn_rows(const AttnArgs &a, const Parts &parts, Split split) {
-    const bool one = a.most * (a.H / a.Hkv) <= 16;
-    if (a.d == 128) return one ? launch_t<128, 1>(a, parts, split) : launch_t<128, 2>(a, parts, split);
-    return one ? launch_t<64, 1>(a, parts, split) : launch_t<64, 2>(a, parts, split);
+    return a.d == 128 ? launch_t<128>(a, parts, split) : launch_t<64>(a, parts, split);
 }
 
 int attn_rows_status(int *flag, bool clear) {

@@ -23,7 +23,13 @@ using namespace attn;
 
 constexpr int THREADS = 256;
 constexpr int KEYS = 64;                       // keys per tile
-constexpr Split SIMT_SPLIT{256, 64}, ROWS_SPLIT{512, 64}, TC_SPLIT{2048, 64};
+// Keys per chunk at least and chunks per sequence at most, by form (64 at most:
+// the join has two per lane). A unit of the tcgen05 form costs some 6 us beside its
+// keys, so its chunks are the longest: one sequence of 131,072 keys took 158 us
+// in chunks of 2,048, 137 us in chunks of 4,096, and 48 trees over caches of
+// U{1..8192} 244 us in chunks of 2,048, 263 us in chunks of 1,024. A warp of the
+// few-row form keeps up with shorter ones (256: 3% more of partial results).
+constexpr Split SIMT_SPLIT{256, 64}, ROWS_SPLIT{512, 64}, TC_SPLIT{2048, 32};
 
 // Four consecutive elements as f32 (d % 4 == 0, 16-byte aligned bases).
 __device__ __forceinline__ float4 get4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
@@ -62,7 +68,7 @@ __device__ Found find_unit(const AttnArgs &a, int64_t x, int tok, Split split) {
         if (i < a.n_seq) {
             const Seq s = seq_of(a, i);
             if (a.paged) chunks = split.chunks(s.keys);
-            units = (s.m + tok - 1) / tok * chunks;
+            units = (static_cast<int64_t>(s.m) + tok - 1) / tok * chunks;
         }
         int64_t incl = units;
 #pragma unroll
@@ -109,10 +115,10 @@ __global__ void __launch_bounds__(THREADS) attn_simt_kernel(const AttnArgs a, co
     const int64_t t0 = static_cast<int64_t>(f.block) * tok;
     const int used = static_cast<int>(min(static_cast<int64_t>(tok), s.m - t0)) * G;
     const int64_t chunks = a.paged ? split.chunks(s.keys) : 1;
-    int64_t kbeg = 0, kend = min(s.keys, s.cached + t0 + tok);
+    int64_t kbeg = 0, kend = min(static_cast<int64_t>(s.keys), s.cached + t0 + tok);
     if (a.paged) {
         if (a.parent) kend = s.keys;
-        kbeg = f.chunk * split.span(s.keys);
+        kbeg = static_cast<int64_t>(f.chunk) * split.span(s.keys);
         kend = min(kend, kbeg + split.span(s.keys));
     }
 

@@ -4,22 +4,34 @@
 //
 // One persistent CTA per SM works through units: 2 x 128 query rows (two
 // tiles) of one (sequence, K/V head), over that pair's keys or a chunk of
-// them, 128 keys at a time:
-//   S_x = Q_x K^T          (tcgen05, both operands in shared memory, f32 in TMEM)
+// them, 64 keys at a time:
+//   S_x = Q_x K^T            (tcgen05, both operands in shared memory, f32 in TMEM)
 //   P_x = exp2(c S_x - c m)  (one warpgroup per tile, a thread per row)
-//   O_x += P_x V           (tcgen05, P as a bf16 A operand in TMEM, over S's columns)
-// with the running maximum m kept lazily: O is rescaled only when a row's
-// maximum has grown by more than 2^8 since m was set, so probabilities stay
-// below 2^8 and the product is rarely interrupted.
+//   O_x += P_x V             (tcgen05, P as a bf16 A operand in TMEM, over S's columns)
+// P is rounded to bf16 because the product takes one type, the type of V; its
+// sum is taken in f32 before the rounding. The maximum m is kept lazily: it is
+// looked for only when a step's sum says that it may have been left behind,
+// and O is rescaled only when it has grown by more than 2^8.
 //
-// Roles: warps 0-3 and 4-7 the softmax of tiles 0 and 1, warp 8 issues every
-// product, warp 9 every copy, warp 10 resolves units ahead of the others.
-// While one tile's softmax runs, the tensor cores work on the other tile. The
-// order PV_x(j), QK_x(j + 1) on the one issuing thread also means that S_x(j)
-// complete implies PV_x(j - 1) complete, so a rescale of O needs no further wait.
+// Roles: warps 0-3 and 4-7 the softmax of tiles 0 and 1, warps 8 and 9 the
+// products of a tile each, warp 10 copies Q and K, warp 11 resolves units ahead
+// of the others and copies V. Scores are held twice per tile, so the order
+// PV_x(e), QK_x(e + 2) lets the tensor cores work on one step while the softmax
+// is on another, and S_x(e + 2) complete implies PV_x(e) complete.
 //
-// What bounds it: 128 x 128 exponentials cost the SM's 16 special-function
-// lanes 1,024 cycles, the two products of a d = 128 tile 1,024 tensor cycles.
+// What bounds it, of a step of 2 x 128 x 64 products at d = 128: the exponentials
+// take the SM's 16 special-function lanes 1,024 cycles, the products 896 of the
+// tensor cores (512 for PV, 384 for QK: 51 cycles each, not 32, as both operands
+// come from shared memory), and the softmax's instructions beside the
+// exponentials share its four schedulers. One prompt of 32,768 tokens (16 heads
+// over 4): 7.8 ms, 1.13 PFLOP/s, 0.70 of a large library product; tensor pipe
+// 75% busy. Steps of 64 keys with P and S held twice took 8.16 ms where steps of
+// 128 took 8.73, an issuing thread per tile and operands in uniform registers
+// 7.86. Measured and not kept, on the 128-key form: part of the exponentials
+// as polynomials on the FMA pipe (9.06 -> 9.30 ms and more with the share), the two tiles
+// taking turns at the exponentials (8.73 -> 8.80 ms).
+// Over the cache with one row tile it is the copies: 4.8 TB/s at 74 sequences
+// of 8,192 keys in pages of 16, where a box of 16 rows is issued every 60 cycles.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -42,9 +54,6 @@ constexpr int KEYS = 64;    // keys of a step
 constexpr int THREADS = 384;
 constexpr int WARP_MMA = 8, WARP_TMA = 10, WARP_SCHED = 11;  // (two of the first)
 constexpr int GROUP = 256;  // sequences whose unit counts the scheduler holds at a time
-#ifndef BATCH
-#define BATCH 8
-#endif
 constexpr float FREE = 65536.f;  // probabilities may reach this against a maximum that was not looked for
 constexpr float LAZY = 8.f; // a row's maximum may grow by 2^LAZY before O is rescaled
 
@@ -98,7 +107,7 @@ struct TcArgs {
     Split split;
     int tok;     // tokens of a row tile: 128 / group
     int group;   // query heads per K/V head
-    int rows;    // rows per TMA box of a paged tile
+    int rows_shift;  // log2 of the rows per TMA box of a paged step
     float c2;    // scale * log2 e
 };
 
@@ -241,7 +250,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t bars = base + C::OFF_BAR, abort = base + C::OFF_MISC + 4;
     Unit *units = reinterpret_cast<Unit *>(smem + C::OFF_UNIT);
     // Keys of a step with memory behind them, 8 bytes a step, 16 steps (K's copies,
-    // which write it, are at most six steps ahead of any softmax that reads).
+    // which write it, are at most two steps more than its ring ahead of any softmax that reads).
     const uint32_t masks = base + C::OFF_MASK;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
     // Unit i of tile x met values that are not finite where not every row sees
@@ -288,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // Units come through a ring of four. The copying and the issuing warp take
+    // Units come through a ring of four. The copying and the issuing warps take
     // theirs out at once, the softmax warps leave it there until they are done.
     auto next_unit = [&](int i, Unit &u) -> bool {
         if (!wait(bars + 8 * (U_FULL + (i & 3)), (i >> 2) & 1, abort)) return false;
@@ -377,20 +386,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const float2 f2 = make_float2(from, from);
                     part[0] = part[1] = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int b = 0; b < 32; b += BATCH) {
-                        float2 y[BATCH];
+                    for (int b = 0; b < 32; b += 8) {
+                        float2 y[8];
 #pragma unroll
-                        for (int k = 0; k < BATCH; ++k) {
+                        for (int k = 0; k < 8; ++k) {
                             const int c = 2 * (b + k);
                             y[k] = fma2(make_float2(v[c / 32][c % 32], v[c / 32][c % 32 + 1]), c2, f2);
                         }
 #pragma unroll
-                        for (int k = 0; k < BATCH; ++k) {
+                        for (int k = 0; k < 8; ++k) {
                             y[k].x = ex2(y[k].x);
                             y[k].y = ex2(y[k].y);
                         }
 #pragma unroll
-                        for (int k = 0; k < BATCH; ++k) {
+                        for (int k = 0; k < 8; ++k) {
                             part[k & 1] = add2(part[k & 1], y[k]);
                             p[b + k] = pack_bf16(y[k].x, y[k].y);
                         }
@@ -487,59 +496,64 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             } else {
                 // Rows leave through the warp's 4 KB of shared memory, 128 bytes of
-                // each at a time, so that eight lanes write a row's whole line: a
-                // thread that writes its own row touches 32 lines per store, and the
-                // 64 KB of a unit took 2,900 cycles that way.
+                // each at a time, so that eight lanes write a row's whole line. The
+                // loops stay rolled: this code runs once in a unit, and fetching
+                // its instructions is most of its time.
+                const bool some = n > 0 && sees;
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const uint32_t mine = used ? static_cast<uint32_t>(split ? g.parts.row(0, row, head) : row * a.H + head) : ~0u;
+                const uint32_t mine = used && some ? static_cast<uint32_t>(split ? g.parts.row(0, row, head) : row * a.H + head) : ~0u;
                 const uint32_t out = base + C::OFF_OUT + warp * 4096;
-                char *dst = (split ? reinterpret_cast<char *>(g.parts.o + g.parts.row(u.chunk, 0, 0) * D) : static_cast<char *>(a.o)) + (lane & 7) * 16;
+                char *dst = split ? reinterpret_cast<char *>(g.parts.o + g.parts.row(u.chunk, 0, 0) * D) : static_cast<char *>(a.o);
                 const int row_bytes = split ? D * 4 : D * 2;
-                auto put = [&](int piece, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((piece ^ (lane & 7)) << 4)),
-                                 "r"(w0), "r"(w1), "r"(w2), "r"(w3)
-                                 : "memory");
-                };
-                uint32_t to_row[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) to_row[k] = __shfl_sync(0xffffffffu, mine, 4 * k + (lane >> 3));
-                auto leave = [&](int at) {  // 128 bytes of every row, from byte `at` of the row
-                    __syncwarp();
-                    uint4 q[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(q[k].x), "=r"(q[k].y), "=r"(q[k].z), "=r"(q[k].w)
-                                     : "r"(out + (4 * k + (lane >> 3)) * 128 + (((lane & 7) ^ ((4 * k + (lane >> 3)) & 7)) << 4)));
-                    __syncwarp();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (to_row[k] != ~0u) *reinterpret_cast<uint4 *>(dst + static_cast<int64_t>(to_row[k]) * row_bytes + at) = q[k];
-                };
+                if (n > 0) {
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    float o[32];
-                    if (n > 0) {
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
                         tmem_ld32(to + c, o);
                         tmem_wait_ld();
-                    }
-                    if (n == 0 || !sees) {
+                        const float2 scale = make_float2(inv, inv), none = make_float2(0.f, 0.f);
+                        uint32_t w[32];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
-                    }
-                    if (split) {
+                        for (int e = 0; e < 16; ++e) {
+                            const float2 y = fma2(make_float2(o[2 * e], o[2 * e + 1]), scale, none);
+                            w[2 * e] = __float_as_uint(y.x);
+                            w[2 * e + 1] = __float_as_uint(y.y);
+                        }
+                        int pieces = 8, at = c * 4, first = 0;
+                        if (!split) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) w[e] = pack_bf16(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+                            pieces = 4;
+                            first = c >> 3 & 4;
+                            at = (c - 32) * 2;
+                        }
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            put(e, __float_as_uint(o[4 * e] * inv), __float_as_uint(o[4 * e + 1] * inv),
-                                __float_as_uint(o[4 * e + 2] * inv), __float_as_uint(o[4 * e + 3] * inv));
-                        leave(c * 4);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            put((c >> 3 & 4) + e, pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
-                        if (c & 32) leave((c - 32) * 2);
+                            if (e < pieces)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + (((first + e) ^ (lane & 7)) << 4)),
+                                             "r"(w[4 * e]), "r"(w[4 * e + 1]), "r"(w[4 * e + 2]), "r"(w[4 * e + 3])
+                                             : "memory");
+                        if (!split && !(c & 32)) continue;
+                        __syncwarp();
+#pragma unroll 2
+                        for (int k = 0; k < 8; ++k) {
+                            const int rr = 4 * k + (lane >> 3);
+                            const uint32_t to_row = __shfl_sync(0xffffffffu, mine, rr);
+                            uint4 q;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                                         : "r"(out + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4))
+                                         : "memory");
+                            if (to_row != ~0u)
+                                *reinterpret_cast<uint4 *>(dst + static_cast<int64_t>(to_row) * row_bytes + at + (lane & 7) * 16) = q;
+                        }
+                        __syncwarp();
                     }
+                }
+                if (used && !some) {  // a row that sees nothing
+                    uint32_t *z = reinterpret_cast<uint32_t *>(dst + (split ? g.parts.row(0, row, head) : row * a.H + head) * row_bytes);
+#pragma unroll 1
+                    for (int c = 0; c < row_bytes / 4; ++c) z[c] = 0u;
                 }
                 if (used) {
                     const float l2 = sum == 0.f ? -INFINITY : top * g.c2 + log2f(sum);
@@ -558,7 +572,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         // warps, one each (a box takes its issuing warp some 60 cycles, and a
         // step has 16 of them where a page is 16 positions; one warp for both
         // needed 1,700 cycles a step). Lane l copies half l % HALVES of page l / HALVES.
-        const int rows = g.rows, pages = KEYS / rows;
+        const int rows = 1 << g.rows_shift, pages = KEYS >> g.rows_shift;
         int ids = -1, page0 = 0;  // the table's entries of 32 pages at a time, a lane each
         int place = 0;            // the first row of this lane's page in the cache
         uint32_t there = 0;       // lanes whose page has memory behind it
@@ -569,7 +583,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 page0 = key >> a.shift;
                 ids = page0 + lane < a.width ? a.block_table[u.seq * a.width + page0 + lane] : -1;
             }
-            const int mine = key + lane / C::HALVES * rows;
+            const int mine = key + (lane / C::HALVES << g.rows_shift);
             const int block = __shfl_sync(0xffffffffu, ids, min(max((mine >> a.shift) - page0, 0), 31));
             const bool has = lane < pages * C::HALVES && mine < u.keys && block >= 0 && block < a.num_blocks;
             there = __ballot_sync(0xffffffffu, has);
@@ -577,10 +591,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         };
         auto copy_step = [&](const Unit &u, int j, uint32_t full, uint32_t dst, const CUtensorMap *tm) {
             if (PAGED) {
-                if (lane == 0) bar_expect(full, __popc(there) * rows * 128);
+                if (lane == 0) bar_expect(full, __popc(there) * (rows * 128));
                 __syncwarp();
                 if (there >> lane & 1u)
-                    load_2d(dst + lane % C::HALVES * (KEYS * 128) + lane / C::HALVES * rows * 128, tm, lane % C::HALVES * 64, place, full);
+                    load_2d(dst + lane % C::HALVES * (KEYS * 128) + (lane / C::HALVES << g.rows_shift) * 128, tm, lane % C::HALVES * 64, place, full);
             } else {
                 if (lane == 0) bar_expect(full, C::TILE);
                 __syncwarp();
@@ -755,7 +769,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                         uint32_t w = ~0u;
                         if (__popc(there) != pages * C::HALVES) {
                             w = 0;
-                            for (int b = 0; b < 32; ++b) w |= (there >> ((lane * 32 + b) / rows * C::HALVES) & 1u) << b;
+#pragma unroll 1
+                            for (int b = 0; b < 32; b += 8)  // (pages are eight positions at least)
+                                w |= (there >> ((lane * 32 + b) >> g.rows_shift) * C::HALVES & 1u) * 0xffu << b;
                         }
                         sts(masks + 8 * (kn & 15) + 4 * lane, w);
                     }
@@ -885,7 +901,7 @@ int launch_t(const AttnArgs &a, const Parts &parts, Split split) {
     g.tok = ROWS / g.group;
     g.c2 = a.scale * LOG2E;
     const int page = 1 << a.shift;
-    g.rows = PAGED && page < KEYS ? page : KEYS;
+    g.rows_shift = PAGED && page < KEYS ? a.shift : 6;
     CUtensorMap tq, tk, tv;
     const uint64_t qd[3] = {D, static_cast<uint64_t>(a.H), static_cast<uint64_t>(a.total_tokens)};
     const uint64_t qs[2] = {D * 2, static_cast<uint64_t>(a.q_stride) * 2};
@@ -898,7 +914,7 @@ int launch_t(const AttnArgs &a, const Parts &parts, Split split) {
         if (PAGED) {
             const uint64_t d[2] = {D, static_cast<uint64_t>(a.num_blocks * a.Hkv) << a.shift};
             const uint64_t s[1] = {D * 2};
-            const uint32_t b[2] = {64, static_cast<uint32_t>(g.rows)};
+            const uint32_t b[2] = {64, 1u << g.rows_shift};
             st = encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B);
         } else {
             const uint64_t d[3] = {D, static_cast<uint64_t>(a.Hkv), static_cast<uint64_t>(a.total_tokens)};

@@ -1179,7 +1179,7 @@ int rhz_attn_tree_fwd(void *o, float *lse, const void *q, const void *k_cache,
     a.paged = true;
     a.block_table = block_table; a.cached = cached; a.parent = parent;
     a.width = width; a.num_blocks = num_blocks; a.shift = shift;
-    a.most = max_positions;
+    a.most = max_positions < INT32_MAX ? max_positions : INT32_MAX;
     a.ws = workspace; a.ws_bytes = workspace_bytes;
     a.stream = as_cuda(stream);
     const size_t need = attn_ws_bytes(a);
@@ -1206,7 +1206,7 @@ size_t rhz_attn_tree_workspace_bytes(int64_t total_tokens, int64_t max_positions
     a.H = H; a.Hkv = H_kv; a.d = d; a.dtype = dtype;
     a.paged = true;
     a.width = width; a.shift = shift;
-    a.most = max_positions;
+    a.most = max_positions < INT32_MAX ? max_positions : INT32_MAX;
     return attn_ws_bytes(a);
 }
 
