@@ -22,26 +22,27 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int MAX_NODES = 64;  // drafted tokens of one sequence (one bit each)
 
-// Splitting the key axis. A paged sequence of L keys is cut into chunks of
-// span(L) keys, anchored at its first key, each computed by itself and joined
+// Splitting the key axis. A paged sequence of L keys is cut into equal chunks
+// of span(L) keys, anchored at its first key, each computed by itself and joined
 // afterwards in order of position. The rule looks at this sequence's length
 // alone, so a sequence's result does not depend on what else is in the batch.
 struct Split {
-    int least;  // keys per chunk at least (a multiple of 128)
-    int most;   // chunks per sequence at most
+    int keys;  // per chunk, where that makes no more than
+    int most;  // chunks of a sequence
     // (Lengths fit 31 bits: the entry refuses wider tables.)
     __host__ __device__ int span(int64_t L) const {
-        const uint32_t c = (static_cast<uint32_t>(L) + most - 1) / most;
-        const int up = static_cast<int>((c + 127) / 128 * 128);
-        return up < least ? least : up;
+        const uint32_t l = static_cast<uint32_t>(L), w = (l + keys - 1) / keys;
+        const uint32_t n = w < 1 ? 1 : w < static_cast<uint32_t>(most) ? w : most;
+        return static_cast<int>((l + n * 128 - 1) / (n * 128) * 128);
     }
     __host__ __device__ int chunks(int64_t L) const {
+        if (L <= keys) return 1;
         const uint32_t c = span(L);
-        return L <= 0 ? 1 : static_cast<int>((static_cast<uint32_t>(L) + c - 1) / c);
+        return static_cast<int>((static_cast<uint32_t>(L) + c - 1) / c);
     }
     // The most chunks that any length up to L can have.
     int64_t bound(int64_t L) const {
-        const int64_t c = (L + least - 1) / least;
+        const int64_t c = (L + keys - 1) / keys;
         return c < 1 ? 1 : (c < most ? c : most);
     }
 };

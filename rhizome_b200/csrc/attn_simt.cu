@@ -23,13 +23,18 @@ using namespace attn;
 
 constexpr int THREADS = 256;
 constexpr int KEYS = 64;                       // keys per tile
-// Keys per chunk at least and chunks per sequence at most, by form (64 at most:
-// the join has two per lane). A unit of the tcgen05 form costs some 6 us beside its
-// keys, so its chunks are the longest: one sequence of 131,072 keys took 158 us
-// in chunks of 2,048, 137 us in chunks of 4,096, and 48 trees over caches of
-// U{1..8192} 244 us in chunks of 2,048, 263 us in chunks of 1,024. A warp of the
-// few-row form keeps up with shorter ones (256: 3% more of partial results).
-constexpr Split SIMT_SPLIT{256, 64}, ROWS_SPLIT{512, 64}, TC_SPLIT{2048, 32};
+constexpr Split SIMT_SPLIT{256, 64}, ROWS_SPLIT{512, 64};
+// Keys per chunk and chunks at most on the tcgen05 form (64 at most: the join
+// has two per lane). A unit costs some 3 us beside its keys, and its rows' partial
+// results are written and read again, so chunks are as long as an even deal
+// allows: 74 trees of 64 nodes over 8,192 keys took 768 us in chunks of 2,048,
+// 706 of 4,096 and 612 of 8,192, but 48 trees over U{1..8192} keys 232, 238
+// and 316. The bound gives one long sequence two units per SM (131,072 keys and
+// 24 nodes: 112 us in 37 chunks, 141 in 32).
+Split tc_split(const AttnArgs &a) {
+    const int most = 2 * 148 / a.Hkv;
+    return {2560, most < 1 ? 1 : most < 64 ? most : 64};
+}
 
 // Four consecutive elements as f32 (d % 4 == 0, 16-byte aligned bases).
 __device__ __forceinline__ float4 get4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
@@ -411,7 +416,7 @@ int launch_simt(const AttnArgs &a, const Parts &parts, Split split) {
 }
 
 Split split_of(const AttnArgs &a) {
-    return attn_rows_supports(a) ? ROWS_SPLIT : attn_tc_supports(a) ? TC_SPLIT : SIMT_SPLIT;
+    return attn_rows_supports(a) ? ROWS_SPLIT : attn_tc_supports(a) ? tc_split(a) : SIMT_SPLIT;
 }
 
 int64_t chunk_bound(const AttnArgs &a) {

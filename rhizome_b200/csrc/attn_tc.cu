@@ -53,7 +53,7 @@ constexpr int ROWS = 128;   // query rows of a tile
 constexpr int KEYS = 64;    // keys of a step
 constexpr int THREADS = 384;
 constexpr int WARP_MMA = 8, WARP_TMA = 10, WARP_SCHED = 11;  // (two of the first)
-constexpr int GROUP = 256;  // sequences whose unit counts the scheduler holds at a time
+constexpr int GROUP = 192;  // sequences whose unit counts the scheduler holds at a time
 constexpr float FREE = 65536.f;  // probabilities may reach this against a maximum that was not looked for
 constexpr float LAZY = 8.f; // a row's maximum may grow by 2^LAZY before O is rescaled
 
@@ -85,7 +85,7 @@ struct Cfg {
     static constexpr int OFF_MASK = OFF_UNIT + 256;
     static constexpr int OFF_MISC = OFF_MASK + 128;
     static constexpr int OFF_COUNT = OFF_MISC + 64;
-    static constexpr int BYTES = OFF_COUNT + GROUP * 4 + 1024;
+    static constexpr int BYTES = OFF_COUNT + GROUP * 5 + 1024;
     static constexpr uint32_t ID_QK = idesc_bf16(ROWS, KEYS, false, false);
     static constexpr uint32_t ID_PV = idesc_bf16(ROWS, D, false, true);
 };
@@ -257,6 +257,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // them: word [x][i & 3] is i + 1. (Unit i + 4 comes when every warp is done with i.)
     const uint32_t spoiled = base + C::OFF_MISC + 16;
     int *counts = reinterpret_cast<int *>(smem + C::OFF_COUNT);
+    uint8_t *costs = reinterpret_cast<uint8_t *>(counts + GROUP);
     const AttnArgs &a = g.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -604,20 +605,24 @@ __global__ void __launch_bounds__(THREADS, 1)
         };
         if (warp == WARP_SCHED) {
             // Resolves units, and copies V.
-            // Units in order of falling cost: unit l of a sequence is its row block
-            // l / chunks (later blocks see more keys), and all sequences' units
-            // of one l come together, the highest l first; dealt to the CTAs in
-            // snake order.
+            // Units in order of falling cost, level by level, dealt to the CTAs in
+            // snake order. Packed: unit l of a sequence is its row block l, which sees
+            // more keys than those before, and a level is all sequences' units of one
+            // l. Paged: a sequence's chunks are equal, and a level is every unit of the
+            // sequences with chunks of this many steps (48 trees over caches of
+            // U{1..8192} keys: 199 us; by the chunks' places alone, which leaves some
+            // CTAs a third more than others, 232 us).
             // (The launch refuses more units than 31 bits count.)
             const int pair = 2 * g.tok, n_seq = static_cast<int>(a.n_seq), G = gridDim.x;
             int before = 0;                          // units of the groups before this one
             int group = -1, total = 0, level = 0;    // of this group: units, current l
             int passed = 0, here = 0;                // units of higher l, sequences with a unit l
+            auto units_at = [&](int j, int l) { return PAGED ? (costs[j] == l ? counts[j] : 0) : static_cast<int>(counts[j] > l); };
             auto at_level = [&](int l) {
                 int n = 0;
 #pragma unroll 1
-                for (int i = lane; i < GROUP; i += 32) n += __popc(__ballot_sync(0xffffffffu, counts[i] > l));
-                return n;
+                for (int j = lane; j < GROUP; j += 32) n += units_at(j, l);
+                return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
             };
             // Unit i of this CTA, passed on to the other roles.
             bool ok = true;
@@ -644,11 +649,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                         int n = 0;
                         if (q < n_seq) {
                             const Seq s = seq_of(a, q);
-                            n = (static_cast<int>(s.m) + pair - 1) / pair * (PAGED ? static_cast<int>(g.split.chunks(s.keys)) : 1);
+                            n = (s.m + pair - 1) / pair * (PAGED ? g.split.chunks(s.keys) : 1);
+                            if (PAGED) {  // a step of one row tile takes three quarters of a step of two
+                                const int steps = min(g.split.span(s.keys) / KEYS, 63);
+                                costs[j] = static_cast<uint8_t>(s.live > g.tok ? steps : steps * 3 / 4);
+                            }
                         }
                         counts[j] = n;
                         total += n;
-                        most = max(most, n);
+                        most = max(most, PAGED ? (n > 0 ? costs[j] + 1 : 0) : n);
                     }
                     total = __reduce_add_sync(0xffffffffu, total);
                     most = __reduce_max_sync(0xffffffffu, most);
@@ -664,37 +673,44 @@ __global__ void __launch_bounds__(THREADS, 1)
                         --level;
                         here = at_level(level);
                     }
-                    int k = want - before - passed;  // the k-th sequence with a unit at this level
+                    int k = want - before - passed;  // unit k of this level, then of its sequence
                     int q = 0;
 #pragma unroll 1
                     for (int j = 0; j < GROUP; j += 32) {
-                        const bool has = counts[j + lane] > level;
-                        const uint32_t b = __ballot_sync(0xffffffffu, has);
-                        if (k < __popc(b)) {
-                            const uint32_t kth = __ballot_sync(0xffffffffu, has && __popc(b & ((1u << lane) - 1u)) == k);
-                            q = group * GROUP + j + __ffs(kth) - 1;
+                        const int mine = units_at(j + lane, level);
+                        int upto = mine;
+#pragma unroll
+                        for (int off = 1; off < 32; off <<= 1) {
+                            const int y = __shfl_up_sync(0xffffffffu, upto, off);
+                            if (lane >= off) upto += y;
+                        }
+                        const uint32_t past = __ballot_sync(0xffffffffu, upto > k);
+                        if (past) {
+                            const int at = __ffs(past) - 1;
+                            q = group * GROUP + j + at;
+                            k -= __shfl_sync(0xffffffffu, upto - mine, at);
                             break;
                         }
-                        k -= __popc(b);
+                        k -= __shfl_sync(0xffffffffu, upto, 31);
                     }
+                    const int l = PAGED ? k : level;  // of the sequence's units
                     const Seq s = seq_of(a, q);
-                    const int keys = static_cast<int>(s.keys), cached = static_cast<int>(s.cached);
-                    const int chunks = PAGED ? static_cast<int>(g.split.chunks(s.keys)) : 1;
+                    const int chunks = PAGED ? g.split.chunks(s.keys) : 1;
                     u.valid = 1;
                     u.seq = q;
                     u.kvh = x - want * a.Hkv;
-                    u.first = static_cast<int>(s.first);
-                    u.m = static_cast<int>(s.m);
-                    u.live = static_cast<int>(s.live);
-                    u.cached = cached;
-                    u.keys = keys;
-                    const int block = level / chunks;
-                    u.chunk = level - block * chunks;
+                    u.first = s.first;
+                    u.m = s.m;
+                    u.live = s.live;
+                    u.cached = s.cached;
+                    u.keys = s.keys;
+                    const int block = l / chunks;
+                    u.chunk = l - block * chunks;
                     u.chunks = chunks;
                     u.t0 = block * pair;
-                    int stop = keys;
+                    int stop = s.keys;
                     if (PAGED) {
-                        const int span = static_cast<int>(g.split.span(s.keys));
+                        const int span = g.split.span(s.keys);
                         u.kbeg = u.chunk * span;
                         stop = min(stop, u.kbeg + span);
                     }
@@ -702,7 +718,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     for (int y = 0; y < 2; ++y) {
                         const int t = u.t0 + y * g.tok;
                         int end = t >= u.live ? 0 : stop;
-                        if (!(PAGED && a.parent)) end = min(end, cached + t + g.tok);
+                        if (!(PAGED && a.parent)) end = min(end, s.cached + t + g.tok);
                         const int steps = max(end - u.kbeg + KEYS - 1, 0) / KEYS;
                         (y ? u.n1 : u.n0) = steps;
                     }
