@@ -1157,9 +1157,9 @@ int rhz_attn_tree_fwd(void *o, float *lse, const void *q, const void *k_cache,
                          (long long)max_positions, (long long)width, (long long)num_blocks);
     if (parent && max_positions > 64)
         return set_error(RHZ_ERR_SHAPE, "a drafted tree has at most 64 positions (got %lld)", (long long)max_positions);
-    if (width << shift > INT32_MAX || num_blocks * H_kv > INT32_MAX >> shift)
-        return set_error(RHZ_ERR_SHAPE, "width * page = %lld positions or num_blocks * H_kv * page = %lld rows: beyond int32 indexing",
-                         (long long)(width << shift), (long long)((num_blocks * H_kv) << shift));
+    if (width > INT32_MAX >> shift || num_blocks > INT32_MAX || num_blocks * H_kv > INT32_MAX >> shift)
+        return set_error(RHZ_ERR_SHAPE, "width = %lld or num_blocks = %lld: width * page positions and num_blocks * H_kv * page rows must fit int32",
+                         (long long)width, (long long)num_blocks);
     RHZ_TRY(check_stride(q_stride, static_cast<int64_t>(H) * d, dtype, "q_stride"));
     if (n_seq == 0 || total_tokens == 0) return RHZ_OK;
     RHZ_TRY(check_ptr(o, "o", 16, true));

@@ -99,6 +99,15 @@ def test_tree_attention_refusals(lib):
     assert w(-1, 8, 4, 16, 8, 4, 32, BF16) == 0 and w(9, 8, 4, 15, 8, 4, 32, BF16) == 0 and w(9, 8, 4, 16, 8, 3, 32, 9) == 0
 
 
+def test_tree_attention_refuses_sizes_whose_products_overflow(lib):
+    names = "o lse q k v table cached cu par n tokens most qs width blocks page H Hkv d scale dt ws wsb stream".split()
+    good = dict.fromkeys(names, FAKE) | dict(n=2, tokens=9, most=8, qs=256, width=4, blocks=10, page=16, H=8, Hkv=4,
+                                             d=32, scale=0.5, dt=BF16, ws=None, wsb=0, stream=None)
+    S = capi.RHZ_ERR_SHAPE
+    refusals(lib.rhz_attn_tree_fwd, names, good, [(S, dict(width=1 << 60)), (S, dict(blocks=1 << 62)),
+                                                  (S, dict(blocks=(1 << 62) + 1))])
+
+
 def test_valid_calls_without_gpu_report_a_device_error(lib):
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
