@@ -383,14 +383,15 @@ int launch_join(const AttnArgs &a, const Parts &parts) {
 
 template <typename T, int ROWS, int NG>
 int launch_simt_t(const AttnArgs &a, const Parts &parts, Split split) {
-    const int smem = 4 * ((ROWS + KEYS) * (a.d + 4) + KEYS * a.d + ROWS * (KEYS + 4));
+    auto bytes = [](int d) { return 4 * ((ROWS + KEYS) * (d + 4) + KEYS * d + ROWS * (KEYS + 4)); };
     const int tok = ROWS / (a.H / a.Hkv);
     const int64_t units = (a.total_tokens / tok + a.n_seq) * parts.most;
     if (units > INT32_MAX) return set_error(RHZ_ERR_SHAPE, "attention over %lld units exceeds the grid", (long long)units);
-    cudaError_t e = cudaFuncSetAttribute(attn_simt_kernel<T, ROWS, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(attn_simt_kernel<T, ROWS, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         bytes(64 * NG));  // for every d, whatever another thread launches
     if (e != cudaSuccess) return set_error(RHZ_ERR_DEVICE, "attn_simt_kernel: %s", cudaGetErrorString(e));
     dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(a.Hkv));
-    attn_simt_kernel<T, ROWS, NG><<<grid, THREADS, smem, a.stream>>>(a, parts, split);
+    attn_simt_kernel<T, ROWS, NG><<<grid, THREADS, bytes(a.d), a.stream>>>(a, parts, split);
     return check_launch("attn_simt_kernel");
 }
 

@@ -706,7 +706,9 @@ int launch_tree_t(const TreeArgs &a) {
     const bool vec = (a.d % 4) == 0;
     auto *kernel = a.d == 32 * NJ ? gdr_tree_kernel<T, NR, NJ, WARPS, true> : gdr_tree_kernel<T, NR, NJ, WARPS, false>;
     const size_t smem = static_cast<size_t>(a.most) * (3 * a.d * sizeof(T) + 3 * 4) + 16;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // The bound of every call of this kernel, so that no thread lowers it under another's launch.
+    constexpr int BOUND = 64 * (3 * 32 * NJ * static_cast<int>(sizeof(T)) + 3 * 4) + 16;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BOUND);
     if (e != cudaSuccess) return set_error(RHZ_ERR_DEVICE, "gdr_tree_kernel: %s", cudaGetErrorString(e));
     kernel<<<grid, WARPS * 32, smem, a.stream>>>(
         static_cast<T *>(a.o), a.states, a.pool, a.slots, a.cu_seqlens, a.parent,
