@@ -304,6 +304,26 @@ def test_many_trees_over_real_caches(d, nodes, H):
                seed=nodes)
 
 
+def test_trees_in_several_scheduling_groups():
+    """Units are ordered by cost in groups of sequences: more than two groups,
+    with sequences of no rows, no cache, one chunk and several."""
+    r = random.Random(5)
+    n = 450
+    check_tree([r.choice([0, 3, 64, 500, 2559, 2560, 2561, 6000]) if r.random() < 0.3 else r.randint(0, 300) for _ in range(n)],
+               [r.choice([0, 1, 5, 17, 33]) for _ in range(n)], 8, 1, 64, BF, seed=5)
+
+
+def test_more_sequences_than_the_few_row_form_holds():
+    r = random.Random(6)
+    n = 4200
+    check_tree([r.randrange(20) for _ in range(n)], [1] * n, 2, 1, 64, BF, page=8, seed=6)
+
+
+@pytest.mark.parametrize("H,Hkv,nodes", [(8, 1, 6), (16, 8, 24)])
+def test_caches_of_the_most_chunks(H, Hkv, nodes):
+    check_tree([170000, 5], [nodes, nodes], H, Hkv, 64, BF, page=64, seed=7)
+
+
 def test_many_prompts_of_mixed_lengths():
     r = random.Random(8)
     check_prompt([r.choice([1, 30, 100, 128, 200, 700]) for _ in range(60)], 16, 4, 128, BF, seed=8)
