@@ -409,8 +409,15 @@ int64_t rows_bound(const AttnArgs &a) {
     return t * (a.H / a.Hkv);
 }
 
+// 16 rows to a CTA where a sequence has no more, or where 64 would leave SMs
+// without work; a row's arithmetic is the same in both, so the batch may choose.
+// f32, d = 32, 2 heads over 1: one prompt of 1,000 tokens 103 us in 64 rows, 55
+// in 16; 8 prompts, 8 over 4: 349 and 508; one of 1,000 with d = 128, 8 over 4, at
+// 128 CTAs of 64 rows: 266 and 253.
 int launch_simt(const AttnArgs &a, const Parts &parts, Split split) {
-    const bool few = rows_bound(a) <= 16;  // (a group of more than 16 heads has more rows)
+    const int group = a.H / a.Hkv;
+    const int64_t wide = (a.total_tokens / (64 / group) + a.n_seq) * parts.most * a.Hkv;  // CTAs of 64 rows, at most
+    const bool few = group <= 16 && (rows_bound(a) <= 16 || wide <= 148);
     if (a.dtype == RHZ_DTYPE_BF16)
         return few ? launch_simt_r<__nv_bfloat16, 16>(a, parts, split) : launch_simt_r<__nv_bfloat16, 64>(a, parts, split);
     return few ? launch_simt_r<float, 16>(a, parts, split) : launch_simt_r<float, 64>(a, parts, split);

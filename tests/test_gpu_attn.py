@@ -110,6 +110,20 @@ def test_prompt_results_do_not_depend_on_the_batch():
         assert torch.equal(alone, o[a:b])
 
 
+@pytest.mark.parametrize("dtype,d", [(F32, 32), (F32, 200), (BF, 96)])
+def test_results_do_not_depend_on_the_rows_of_a_tile(dtype, d):
+    """A call of little work takes smaller row tiles: the same bits."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    counts = [70, 0, 333, 1] + [250] * 40
+    at, cu = cu_of(counts)
+    q = torch.randn(at[-1], 6, d, generator=g, device="cuda").to(dtype)
+    k = torch.randn(at[-1], 2, d, generator=g, device="cuda").to(dtype)
+    v = torch.randn(at[-1], 2, d, generator=g, device="cuda").to(dtype)
+    o = ops.attn_varlen_fwd(q, k, v, cu)
+    for a, b in list(zip(at, at[1:]))[:6]:
+        assert torch.equal(ops.attn_varlen_fwd(q[a:b], k[a:b], v[a:b], cu_of([b - a])[1]), o[a:b])
+
+
 # ------------------------------------------------------------------ the paged cache
 
 class Paged:
