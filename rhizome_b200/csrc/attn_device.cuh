@@ -1,6 +1,6 @@
 // What the two tensor-core forms of the attention share on the device:
 // barriers and copies by 32-bit shared-memory addresses, the bits of the keys
-// that a row sees, and the plain-arithmetic form of one row.
+// that a row sees, and values that are not finite.
 #pragma once
 
 #include <cuda.h>
@@ -86,28 +86,38 @@ __device__ __forceinline__ uint32_t seen_word(int all, uint64_t bits, int start)
     return n > -64 ? static_cast<uint32_t>(bits >> -n) : 0u;
 }
 
-// Where a row's keys are and its result goes.
+// Where a unit's keys are and its results go.
 struct RowPlace {
-    int seq, kvh, first, kbeg, kend, chunk, chunks;
+    int seq, kvh, first, chunk, chunks;
 };
 
-// One row by plain arithmetic from global memory, a warp per row: for tiles
-// that hold values which are not finite where some rows must not see them
-// (the tensor cores' 0 * NaN would reach every row of the tile).
+// Whether one of the two bf16 in a word is not finite, and the word without
+// those that are not.
+__device__ __forceinline__ bool odd_word(uint32_t w) {
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+__device__ __forceinline__ uint32_t finite_word(uint32_t w) {
+    if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+    if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
+    return w;
+}
+
+// Values that are not finite at keys that not every row of a tile sees. The
+// tensor cores' 0 * NaN would take them to every row, so the kernels replace
+// them by zero in shared memory and, once a unit's rows are written, come here
+// for the keys [from, to) that this can be (128 of them and a step at most).
+// What a row that sees such a key has to get follows without its probability:
+// that is positive, so an infinity stays one, and what was written is finite
+// there or not finite already. Only where the key's score is itself not finite
+// (its K row is not) it is 0 * inf or worse, a NaN. A lane of the warp has one
+// row: token * H + head, with `takes` false where it sees no key at all.
 template <int D>
-__device__ __noinline__ void plain_row(const AttnArgs &a, const Parts &parts, float c2, const RowPlace at, int t, int of_group,
-                                       const Sight sight, int lane) {
-    constexpr int C = D / 32;  // channels of a lane
-    const int64_t token = at.first + t;
-    const int head = at.kvh * (a.H / a.Hkv) + of_group;
-    const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.q) + token * a.q_stride + static_cast<int64_t>(head) * D + lane * C;
-    float qx[C], acc[C], top = -INFINITY, sum = 0.f;
-    for (int e = 0; e < C; ++e) {
-        qx[e] = __bfloat162float(q[e]);
-        acc[e] = 0.f;
-    }
-    for (int key = at.kbeg; key < at.kend; ++key) {
-        if (!sight.sees(key)) continue;
+__device__ __noinline__ void add_odd_values(const AttnArgs &a, const Parts &parts, const RowPlace at, int from, int to, bool takes,
+                                            uint32_t row, int all, uint64_t bits, int lane) {
+    constexpr int W = D / 64;  // words of a lane
+    const Sight sight{all, bits};
+    __syncwarp();  // the rows were written by other lanes of this warp
+    for (int key = from; key < to; ++key) {
         int64_t kat, vat;
         if (a.paged) {
             const int64_t block = a.block_table[at.seq * a.width + (key >> a.shift)];
@@ -117,27 +127,34 @@ __device__ __noinline__ void plain_row(const AttnArgs &a, const Parts &parts, fl
             kat = (static_cast<int64_t>(at.first) + key) * a.k_stride + static_cast<int64_t>(at.kvh) * D;
             vat = (static_cast<int64_t>(at.first) + key) * a.v_stride + static_cast<int64_t>(at.kvh) * D;
         }
-        float s = 0.f;
-        for (int e = 0; e < C; ++e) s = fmaf(qx[e], __bfloat162float(static_cast<const __nv_bfloat16 *>(a.k)[kat + lane * C + e]), s);
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        s *= c2;
-        const float best = fmaxf(top, s), from = best == -INFINITY ? 0.f : best;
-        const float keep = ex2(top - from), p = ex2(s - from);
-        top = best;
-        sum = sum * keep + p;
-        for (int e = 0; e < C; ++e)
-            acc[e] = fmaf(p, __bfloat162float(static_cast<const __nv_bfloat16 *>(a.v)[vat + lane * C + e]), acc[e] * keep);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const float l2 = sum == 0.f ? -INFINITY : top + log2f(sum);
-    if (at.chunks > 1) {
-        const int64_t r = parts.row(at.chunk, token, head);
-        if (lane == 0) parts.lse[r] = l2;
-        for (int e = 0; e < C; ++e) parts.o[r * D + lane * C + e] = acc[e] * inv;
-    } else {
-        if (lane == 0 && a.lse) a.lse[token * a.H + head] = l2 * LN2;
-        for (int e = 0; e < C; ++e)
-            static_cast<__nv_bfloat16 *>(a.o)[(token * a.H + head) * D + lane * C + e] = __float2bfloat16_rn(acc[e] * inv);
+        const uint32_t *kw = reinterpret_cast<const uint32_t *>(static_cast<const __nv_bfloat16 *>(a.k) + kat) + lane * W;
+        const uint32_t *vw = reinterpret_cast<const uint32_t *>(static_cast<const __nv_bfloat16 *>(a.v) + vat) + lane * W;
+        uint32_t v[W];
+        bool odd = false, odd_k = false;
+        for (int e = 0; e < W; ++e) {
+            v[e] = vw[e];
+            odd |= odd_word(v[e]);
+            odd_k |= odd_word(kw[e]);
+        }
+        if (!__any_sync(0xffffffffu, odd)) continue;
+        odd_k = __any_sync(0xffffffffu, odd_k);
+        for (uint32_t who = __ballot_sync(0xffffffffu, takes && sight.sees(key)); who != 0; who &= who - 1) {
+            const uint32_t to_row = __shfl_sync(0xffffffffu, row, __ffs(who) - 1);
+            if (!odd) continue;
+            for (int c = 0; c < 2 * W; ++c) {
+                const float x = __uint_as_float(c & 1 ? v[c >> 1] & 0xffff0000u : v[c >> 1] << 16);
+                if (isfinite(x)) continue;
+                const float add = odd_k ? NAN : x;
+                const int64_t place = static_cast<int64_t>(to_row) * D + lane * 2 * W + c;
+                if (at.chunks > 1) {
+                    float *o = parts.o + parts.row(at.chunk, 0, 0) * D + place;
+                    *o += add;
+                } else {
+                    __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(a.o) + place;
+                    *o = __float2bfloat16_rn(__bfloat162float(*o) + add);
+                }
+            }
+        }
     }
 }
 

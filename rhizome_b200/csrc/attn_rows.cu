@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
             const uint32_t valid = lds(valid_at + 4 * st);
             const bool edge = valid != ~0u || key + KEYS > full;
             if (edge) {
-                // V of keys behind the sequence or without a page becomes zero;
-                // values that are not finite where not every row looks are noted.
+                // V of keys behind the sequence or without a page becomes zero, and so do
+                // values that are not finite where not every row looks; those are noted.
                 const bool exists = key + lane < end && (valid >> lane & 1u);
                 if (!exists || key + lane >= full) {
                     for (int c = 0; c < D / 8; ++c) {
@@ -311,8 +311,12 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
                                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                                          : "r"(at)
                                          : "memory");
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
+                            if (odd_word(w[0]) || odd_word(w[1]) || odd_word(w[2]) || odd_word(w[3])) {
+                                bad = true;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(finite_word(w[0])),
+                                             "r"(finite_word(w[1])), "r"(finite_word(w[2])), "r"(finite_word(w[3]))
+                                             : "memory");
+                            }
                         }
                     }
                 }
@@ -395,7 +399,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
             copy(k);
         }
         if (!ok) break;
-        bad = __any_sync(0xffffffffu, bad);
+        bool some[2];  // rows that see a key
         const bool split = u.chunks > 1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -404,9 +408,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             const int r = gq + 8 * i, t = r / g.group, of = r - t * g.group;
             if (all[i] == 0 && bits[i] == 0) l = 0.f;  // sees nothing: whole tiles did not ask
+            some[i] = r < used && l != 0.f;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const float l2 = l == 0.f ? -INFINITY : top[i] + log2f(l);
-            if (r >= used || bad) continue;
+            if (r >= used) continue;
             const int64_t token = u.first + t;
             const int head = u.kvh * g.group + of;
             if (split) {
@@ -425,18 +430,18 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
                     dst[4 * n] = l == 0.f ? 0u : pack_bf16(acc[n][2 * i] * inv, acc[n][2 * i + 1] * inv);
             }
         }
-        if (bad) {
-            for (int r = 0; r < used; ++r) {
-                const int t = r / g.group;
-                Sight s{0, 0};
-                if (a.parent) {
-                    s.bits = ancestors(a.parent + u.first, t);
-                    s.all = s.bits ? u.cached : 0;
-                } else {
-                    s.all = u.cached + t + 1;
-                }
-                plain_row<D>(a, g.parts, g.c2, {u.seq, u.kvh, u.first, u.kbeg, u.kend, u.chunk, u.chunks}, t, r - t * g.group, s, lane);
-            }
+        if (__any_sync(0xffffffffu, bad)) {
+            // Lane r takes row r, from a lane that holds it.
+            const int from = 4 * (lane & 7), i = lane >> 3 & 1;
+            const int all0 = __shfl_sync(0xffffffffu, all[0], from), all1 = __shfl_sync(0xffffffffu, all[1], from);
+            const uint64_t bits0 = __shfl_sync(0xffffffffu, bits[0], from), bits1 = __shfl_sync(0xffffffffu, bits[1], from);
+            const int some0 = __shfl_sync(0xffffffffu, static_cast<int>(some[0]), from);
+            const int some1 = __shfl_sync(0xffffffffu, static_cast<int>(some[1]), from);
+            const int r = lane & 15, t = r / g.group;
+            add_odd_values<D>(a, g.parts, {u.seq, u.kvh, u.first, u.chunk, u.chunks}, max(full, u.kbeg), end,
+                              lane < 16 && (i ? some1 : some0) != 0,
+                              static_cast<uint32_t>(u.first + t) * a.H + u.kvh * g.group + (r - t * g.group), i ? all1 : all0,
+                              i ? bits1 : bits0, lane);
         }
         if (u.chunk == 0) {
             if (g.parts.count && u.kvh == 0)

@@ -208,8 +208,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // V of a step that not every row sees whole, a step's 64 keys by a warpgroup,
 // two threads to a key: rows behind the sequence or without a page become
-// zero, and values that are not finite in rows from key `full` on are noted
-// at `spoiled`. (A probability of zero does not keep them out of a product.)
+// zero, and so do values that are not finite at keys from `full` on, which are
+// noted at `spoiled`. (A probability of zero does not keep them out of a
+// product.) Both row tiles read these keys, so `full` is the unit's, and each
+// tile's warpgroup cleans every such step before its own product. What one has
+// replaced the other no longer finds, so the note comes first.
 template <int D, bool PAGED>
 __device__ __forceinline__ void clean_values(uint32_t tile, uint32_t mask, int key, int keys, int full, int r,
                                              uint32_t spoiled, int mark) {
@@ -217,7 +220,6 @@ __device__ __forceinline__ void clean_values(uint32_t tile, uint32_t mask, int k
     const uint32_t vrow = tile + kr * 128 + (D == 128 ? (r & 1) * (KEYS * 128) : 0);
     const bool exists = key + kr < keys && (!PAGED || (lds(mask + 4 * (kr >> 5)) >> (kr & 31) & 1u));
     if (!exists || key + kr >= full) {
-        bool bad = false;
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {  // 16-byte pieces; lanes start at different ones: different banks
             const int piece = D == 128 ? ((c + kr) & 7) : ((c + kr) & 3) + 4 * (r & 1);
@@ -230,11 +232,15 @@ __device__ __forceinline__ void clean_values(uint32_t tile, uint32_t mask, int k
                              : "=r"(ws[0]), "=r"(ws[1]), "=r"(ws[2]), "=r"(ws[3])
                              : "r"(at)
                              : "memory");
-#pragma unroll
-                for (int k = 0; k < 4; ++k) bad |= (ws[k] & 0x7f80u) == 0x7f80u || (ws[k] & 0x7f800000u) == 0x7f800000u;
+                if (odd_word(ws[0]) || odd_word(ws[1]) || odd_word(ws[2]) || odd_word(ws[3])) {
+                    sts(spoiled, mark);
+                    __threadfence_block();
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(finite_word(ws[0])), "r"(finite_word(ws[1])),
+                                 "r"(finite_word(ws[2])), "r"(finite_word(ws[3]))
+                                 : "memory");
+                }
             }
         }
-        if (bad) sts(spoiled, mark);
     }
     fence_proxy_async_smem();
 }
@@ -253,8 +259,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     // which write it, are at most two steps more than its ring ahead of any softmax that reads).
     const uint32_t masks = base + C::OFF_MASK;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
-    // Unit i of tile x met values that are not finite where not every row sees
-    // them: word [x][i & 3] is i + 1. (Unit i + 4 comes when every warp is done with i.)
+    // Unit i met values that are not finite where not every row sees them: word
+    // i & 3 is i + 1. (Unit i + 4 comes when every warp is done with i.)
     const uint32_t spoiled = base + C::OFF_MISC + 16;
     int *counts = reinterpret_cast<int *>(smem + C::OFF_COUNT);
     uint8_t *costs = reinterpret_cast<uint8_t *>(counts + GROUP);
@@ -284,7 +290,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         bar_init(bars + 8 * DRAIN, 2);
         sts(abort, 0);
-        for (int i = 0; i < 8; ++i) sts(spoiled + 4 * i, 0);
+        for (int i = 0; i < 4; ++i) sts(spoiled + 4 * i, 0);
         mbar_fence_init();
     }
     if (warp == WARP_MMA) tmem_alloc(tmem_slot, 512);
@@ -335,6 +341,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             // Tiles below `full` are seen whole by every live row of the warpgroup's tile.
             const int full = PAGED && a.parent ? u.cached : u.cached + u.t0 + x * g.tok + 1;
+            auto full_both = [&]() { return u.cached + (PAGED && a.parent ? 0 : u.t0 + 1); };  // and by those of both tiles
             const int kbeg = u.kbeg;
             const bool sees = all > 0 || bits != 0;  // (rows that do not are computed and thrown away)
             float top = -INFINITY, sum = 0.f;
@@ -342,6 +349,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int n = x ? u.n1 : u.n0;
             // Halves that every live row sees whole.
             const int whole = min(max(full - kbeg, 0) / KEYS, n);
+            const int clean = max(full_both() - kbeg, 0) / KEYS;  // steps before this one need no clean_values
             bool loaded = false;  // v holds step e's scores
             float v[2][32];
             auto load = [&](int h) {
@@ -366,14 +374,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                                  : "memory");
                     edge |= (there[0] & there[1]) != ~0u;
                 }
-                if (edge) {
+                if (edge || e >= clean) {
                     // Not before the scores are there: only then is V's place in the ring
                     // at most one lap from its turn, and the parity tells. (A warpgroup
                     // without steps in a unit runs ahead of the ring.)
                     const int vs = nth % C::STAGES;
                     ok = wait(bars + 8 * (V_FULL + vs), (nth / C::STAGES) & 1, abort);
                     if (!ok) break;
-                    clean_values<D, PAGED>(base + C::OFF_V + vs * C::TILE, masks + 8 * (nth & 15), key, u.keys, full, r, spoiled + 16 * x + 4 * (i & 3), i + 1);
+                    clean_values<D, PAGED>(base + C::OFF_V + vs * C::TILE, masks + 8 * (nth & 15), key, u.keys, full_both(), r, spoiled + 4 * (i & 3), i + 1);
                 }
                 tmem_wait_ld();
                 sp ^= 1u << h;
@@ -480,88 +488,80 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!wait(bars + 8 * (O_FULL + x), on & 1, abort)) break;
                 ++on;
                 tc_fence_after();
-                bad = lds(spoiled + 16 * x + 4 * (i & 3)) == i + 1;  // written before its warp's last p_full arrival
+                bad = lds(spoiled + 4 * (i & 3)) == i + 1;  // written before this tile's P of that step was handed over
             }
             if (!sees) sum = 0.f;
             const int64_t row = u.first + token;
             const int head = u.kvh * g.group + row_head;
             const bool split = PAGED && u.chunks > 1;
-            if (bad) {
-                const int kend = min(u.keys, u.kbeg + n * KEYS);
-                for (int w = 0; w < 32; ++w) {  // the warp takes its own 32 rows
-                    const int rr = (warp & 3) * 32 + w;
-                    const Sight theirs{__shfl_sync(0xffffffffu, all, w), __shfl_sync(0xffffffffu, bits, w)};
-                    if (__shfl_sync(0xffffffffu, static_cast<int>(used), w))
-                        plain_row<D>(a, g.parts, g.c2, {u.seq, u.kvh, u.first, u.kbeg, kend, u.chunk, u.chunks}, u.t0 + x * g.tok + rr / g.group,
-                                     rr % g.group, theirs, lane);
-                }
-            } else {
-                // Rows leave through the warp's 4 KB of shared memory, 128 bytes of
-                // each at a time, so that eight lanes write a row's whole line. The
-                // loops stay rolled: this code runs once in a unit, and fetching
-                // its instructions is most of its time.
-                const bool some = n > 0 && sees;
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const uint32_t mine = used && some ? static_cast<uint32_t>(split ? g.parts.row(0, row, head) : row * a.H + head) : ~0u;
-                const uint32_t out = base + C::OFF_OUT + warp * 4096;
-                char *dst = split ? reinterpret_cast<char *>(g.parts.o + g.parts.row(u.chunk, 0, 0) * D) : static_cast<char *>(a.o);
-                const int row_bytes = split ? D * 4 : D * 2;
-                if (n > 0) {
+            // Rows leave through the warp's 4 KB of shared memory, 128 bytes of
+            // each at a time, so that eight lanes write a row's whole line. The
+            // loops stay rolled: this code runs once in a unit, and fetching
+            // its instructions is most of its time.
+            const bool some = n > 0 && sees;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const uint32_t mine = used && some ? static_cast<uint32_t>(split ? g.parts.row(0, row, head) : row * a.H + head) : ~0u;
+            const uint32_t out = base + C::OFF_OUT + warp * 4096;
+            char *dst = split ? reinterpret_cast<char *>(g.parts.o + g.parts.row(u.chunk, 0, 0) * D) : static_cast<char *>(a.o);
+            const int row_bytes = split ? D * 4 : D * 2;
+            if (n > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        tmem_ld32(to + c, o);
-                        tmem_wait_ld();
-                        const float2 scale = make_float2(inv, inv), none = make_float2(0.f, 0.f);
-                        uint32_t w[32];
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    tmem_ld32(to + c, o);
+                    tmem_wait_ld();
+                    const float2 scale = make_float2(inv, inv), none = make_float2(0.f, 0.f);
+                    uint32_t w[32];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float2 y = fma2(make_float2(o[2 * e], o[2 * e + 1]), scale, none);
-                            w[2 * e] = __float_as_uint(y.x);
-                            w[2 * e + 1] = __float_as_uint(y.y);
-                        }
-                        int pieces = 8, at = c * 4, first = 0;
-                        if (!split) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) w[e] = pack_bf16(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
-                            pieces = 4;
-                            first = c >> 3 & 4;
-                            at = (c - 32) * 2;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (e < pieces)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + (((first + e) ^ (lane & 7)) << 4)),
-                                             "r"(w[4 * e]), "r"(w[4 * e + 1]), "r"(w[4 * e + 2]), "r"(w[4 * e + 3])
-                                             : "memory");
-                        if (!split && !(c & 32)) continue;
-                        __syncwarp();
-#pragma unroll 2
-                        for (int k = 0; k < 8; ++k) {
-                            const int rr = 4 * k + (lane >> 3);
-                            const uint32_t to_row = __shfl_sync(0xffffffffu, mine, rr);
-                            uint4 q;
-                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                         : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
-                                         : "r"(out + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4))
-                                         : "memory");
-                            if (to_row != ~0u)
-                                *reinterpret_cast<uint4 *>(dst + static_cast<int64_t>(to_row) * row_bytes + at + (lane & 7) * 16) = q;
-                        }
-                        __syncwarp();
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 y = fma2(make_float2(o[2 * e], o[2 * e + 1]), scale, none);
+                        w[2 * e] = __float_as_uint(y.x);
+                        w[2 * e + 1] = __float_as_uint(y.y);
                     }
-                }
-                if (used && !some) {  // a row that sees nothing
-                    uint32_t *z = reinterpret_cast<uint32_t *>(dst + (split ? g.parts.row(0, row, head) : row * a.H + head) * row_bytes);
-#pragma unroll 1
-                    for (int c = 0; c < row_bytes / 4; ++c) z[c] = 0u;
-                }
-                if (used) {
-                    const float l2 = sum == 0.f ? -INFINITY : top * g.c2 + log2f(sum);
-                    if (split) g.parts.lse[g.parts.row(u.chunk, row, head)] = l2;
-                    else if (a.lse) a.lse[row * a.H + head] = l2 * LN2;
+                    int pieces = 8, at = c * 4, first = 0;
+                    if (!split) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) w[e] = pack_bf16(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+                        pieces = 4;
+                        first = c >> 3 & 4;
+                        at = (c - 32) * 2;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < pieces)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + (((first + e) ^ (lane & 7)) << 4)),
+                                         "r"(w[4 * e]), "r"(w[4 * e + 1]), "r"(w[4 * e + 2]), "r"(w[4 * e + 3])
+                                         : "memory");
+                    if (!split && !(c & 32)) continue;
+                    __syncwarp();
+#pragma unroll 2
+                    for (int k = 0; k < 8; ++k) {
+                        const int rr = 4 * k + (lane >> 3);
+                        const uint32_t to_row = __shfl_sync(0xffffffffu, mine, rr);
+                        uint4 q;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                                     : "r"(out + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4))
+                                     : "memory");
+                        if (to_row != ~0u)
+                            *reinterpret_cast<uint4 *>(dst + static_cast<int64_t>(to_row) * row_bytes + at + (lane & 7) * 16) = q;
+                    }
+                    __syncwarp();
                 }
             }
+            if (used && !some) {  // a row that sees nothing
+                uint32_t *z = reinterpret_cast<uint32_t *>(dst + (split ? g.parts.row(0, row, head) : row * a.H + head) * row_bytes);
+#pragma unroll 1
+                for (int c = 0; c < row_bytes / 4; ++c) z[c] = 0u;
+            }
+            if (used) {
+                const float l2 = sum == 0.f ? -INFINITY : top * g.c2 + log2f(sum);
+                if (split) g.parts.lse[g.parts.row(u.chunk, row, head)] = l2;
+                else if (a.lse) a.lse[row * a.H + head] = l2 * LN2;
+            }
+            if (bad)
+                add_odd_values<D>(a, g.parts, {u.seq, u.kvh, u.first, u.chunk, u.chunks}, max(full_both(), kbeg), min(u.keys, kbeg + n * KEYS),
+                                  used && sum != 0.f, static_cast<uint32_t>(row * a.H + head), all, bits, lane);
             if (PAGED && used && g.parts.count && u.chunk == 0 && head == 0) g.parts.count[row] = u.chunks;
             tc_fence_before();
             __syncwarp();
