@@ -442,7 +442,8 @@ int rhz_kv_append(void *k_cache, void *v_cache, const void *k, const void *v,
  *   lse_t = log sum_j exp(s_j)
  * q [tokens][H][d], k and v [tokens][H_kv][d], rows q_stride, k_stride,
  * v_stride elements apart (multiples of 8 for bf16, 4 for f32, 16-byte
- * aligned bases); o [tokens][H][d] contiguous; lse [tokens][H] f32 or NULL.
+ * aligned bases); o [tokens][H][d] contiguous; lse [tokens][H] f32 or NULL;
+ * at most 2^22 sequences (empty ones count).
  * Rows outside [cu_seqlens[0], cu_seqlens[n_seq]) are left as they were.
  * Values of rows that a row does not see never reach it, NaN and infinities
  * included. H a multiple of H_kv, at most 64 query heads to a K/V head; d a

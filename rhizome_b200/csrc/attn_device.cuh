@@ -34,6 +34,14 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// The limit of a wait, 2 s by the card's clock (its low word: differences are
+// good to 4 s), looked at every 64 tries.
+constexpr uint32_t WAIT_NS = 2000000000u;
+__device__ __forceinline__ uint32_t clock_ns() {
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+    return t;
+}
 __device__ __forceinline__ uint32_t lds(uint32_t at) {
     uint32_t x;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
@@ -87,8 +95,8 @@ __device__ __forceinline__ uint32_t seen_word(int all, uint64_t bits, int start)
 }
 
 // Where a unit's keys are and its results go.
-struct RowPlace {
-    int seq, kvh, first, chunk, chunks;
+struct Place {
+    int seq, kvh, chunk, chunks;
 };
 
 // Whether one of the two bf16 in a word is not finite, and the word without
@@ -110,12 +118,14 @@ __device__ __forceinline__ uint32_t finite_word(uint32_t w) {
 // that is positive, so an infinity stays one, and what was written is finite
 // there or not finite already. Only where the key's score is itself not finite
 // (its K row is not) it is 0 * inf or worse, a NaN. A lane of the warp has one
-// row: token * H + head, with `takes` false where it sees no key at all.
+// row: token t of the sequence and a head, with `takes` false where it is none
+// or sees no key at all.
 template <int D>
-__device__ __noinline__ void add_odd_values(const AttnArgs &a, const Parts &parts, const RowPlace at, int from, int to, bool takes,
-                                            uint32_t row, int all, uint64_t bits, int lane) {
+__device__ __noinline__ void add_odd_values(const AttnArgs &a, const Parts &parts, const Seq s, const Place at, int from, int to, bool takes,
+                                            int t, int head, int lane) {
     constexpr int W = D / 64;  // words of a lane
-    const Sight sight{all, bits};
+    const Sight sight = takes ? sight_of(a, s, t) : Sight{0, 0};
+    const uint32_t row = static_cast<uint32_t>(s.first + t) * a.H + head;
     __syncwarp();  // the rows were written by other lanes of this warp
     for (int key = from; key < to; ++key) {
         int64_t kat, vat;
@@ -124,8 +134,8 @@ __device__ __noinline__ void add_odd_values(const AttnArgs &a, const Parts &part
             if (block < 0 || block >= a.num_blocks) continue;
             kat = vat = (((block * a.Hkv + at.kvh) << a.shift) + (key & ((1 << a.shift) - 1))) * D;
         } else {
-            kat = (static_cast<int64_t>(at.first) + key) * a.k_stride + static_cast<int64_t>(at.kvh) * D;
-            vat = (static_cast<int64_t>(at.first) + key) * a.v_stride + static_cast<int64_t>(at.kvh) * D;
+            kat = (static_cast<int64_t>(s.first) + key) * a.k_stride + static_cast<int64_t>(at.kvh) * D;
+            vat = (static_cast<int64_t>(s.first) + key) * a.v_stride + static_cast<int64_t>(at.kvh) * D;
         }
         const uint32_t *kw = reinterpret_cast<const uint32_t *>(static_cast<const __nv_bfloat16 *>(a.k) + kat) + lane * W;
         const uint32_t *vw = reinterpret_cast<const uint32_t *>(static_cast<const __nv_bfloat16 *>(a.v) + vat) + lane * W;

@@ -286,8 +286,11 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
         for (int key = u.kbeg; key < end; key += KEYS, ++tile) {
             const int st = tile % STAGES;
             const uint32_t bar = bars + 8 * st;
-            bool came = false;
-            for (uint32_t i = 0; i < (1u << 21) && !came; ++i) came = bar_try(bar, (tile / STAGES) & 1);
+            bool came = bar_try(bar, (tile / STAGES) & 1);
+            if (!came) {
+                const uint32_t since = clock_ns();
+                for (uint32_t i = 1; !came && ((i & 63u) != 0 || clock_ns() - since <= WAIT_NS); ++i) came = bar_try(bar, (tile / STAGES) & 1);
+            }
             ok = __all_sync(0xffffffffu, came);
             if (!ok) {
                 atomicExch(&g_rows_timeout, 1);
@@ -431,17 +434,11 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
             }
         }
         if (__any_sync(0xffffffffu, bad)) {
-            // Lane r takes row r, from a lane that holds it.
-            const int from = 4 * (lane & 7), i = lane >> 3 & 1;
-            const int all0 = __shfl_sync(0xffffffffu, all[0], from), all1 = __shfl_sync(0xffffffffu, all[1], from);
-            const uint64_t bits0 = __shfl_sync(0xffffffffu, bits[0], from), bits1 = __shfl_sync(0xffffffffu, bits[1], from);
-            const int some0 = __shfl_sync(0xffffffffu, static_cast<int>(some[0]), from);
-            const int some1 = __shfl_sync(0xffffffffu, static_cast<int>(some[1]), from);
-            const int r = lane & 15, t = r / g.group;
-            add_odd_values<D>(a, g.parts, {u.seq, u.kvh, u.first, u.chunk, u.chunks}, max(full, u.kbeg), end,
-                              lane < 16 && (i ? some1 : some0) != 0,
-                              static_cast<uint32_t>(u.first + t) * a.H + u.kvh * g.group + (r - t * g.group), i ? all1 : all0,
-                              i ? bits1 : bits0, lane);
+            const int r = lane & 15, t = r / g.group;  // lane r takes row r
+            const bool some0 = __shfl_sync(0xffffffffu, static_cast<int>(some[0]), 4 * (lane & 7));
+            const bool some1 = __shfl_sync(0xffffffffu, static_cast<int>(some[1]), 4 * (lane & 7));
+            add_odd_values<D>(a, g.parts, {u.first, u.m, u.live, u.cached, u.cached + u.live}, {u.seq, u.kvh, u.chunk, u.chunks},
+                              max(full, u.kbeg), end, lane < 16 && (lane & 8 ? some1 : some0), t, u.kvh * g.group + (r - t * g.group), lane);
         }
         if (u.chunk == 0) {
             if (g.parts.count && u.kvh == 0)

@@ -144,13 +144,16 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_l
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// Bounded wait of one thread (2^21 tries, some 0.1 to 2 s) that also ends when
-// another role gave up; *stop in shared memory tells the others.
+// Bounded wait of one thread (WAIT_NS) that also ends when another role gave up;
+// *stop in shared memory tells the others.
 __device__ __forceinline__ bool wait1(uint32_t bar, uint32_t parity, uint32_t stop) {
+    uint32_t since = 0;
     for (uint32_t i = 0; !bar_try(bar, parity); ++i) {
         if ((i & 63u) != 63u) continue;
         if (lds(stop) != 0) return false;
-        if (i >= (1u << 21)) {
+        const uint32_t now = clock_ns();
+        if (i == 63u) since = now;
+        if (now - since > WAIT_NS) {
             sts(stop, 1);
             atomicExch(&g_attn_timeout, 1);
             return false;
@@ -559,10 +562,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (split) g.parts.lse[g.parts.row(u.chunk, row, head)] = l2;
                 else if (a.lse) a.lse[row * a.H + head] = l2 * LN2;
             }
-            if (bad)
-                add_odd_values<D>(a, g.parts, {u.seq, u.kvh, u.first, u.chunk, u.chunks}, max(full_both(), kbeg), min(u.keys, kbeg + n * KEYS),
-                                  used && sum != 0.f, static_cast<uint32_t>(row * a.H + head), all, bits, lane);
             if (PAGED && used && g.parts.count && u.chunk == 0 && head == 0) g.parts.count[row] = u.chunks;
+            if (bad)
+                add_odd_values<D>(a, g.parts, {u.first, u.m, u.live, u.cached, u.keys}, {u.seq, u.kvh, u.chunk, u.chunks},
+                                  max(full_both(), kbeg), min(u.keys, kbeg + n * KEYS), used && sum != 0.f, token, head, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(bars + 8 * (U_EMPTY + (i & 3)));

@@ -1035,7 +1035,9 @@ int check_stride(int64_t stride, int64_t row, int32_t dtype, const char *name) {
 int check_attn_sizes(int64_t n_seq, int64_t total_tokens, int32_t H) {
     if (n_seq < 0 || total_tokens < 0)
         return set_error(RHZ_ERR_SHAPE, "negative size (n_seq %lld, total_tokens %lld)", (long long)n_seq, (long long)total_tokens);
-    if (n_seq > INT32_MAX - 1 || total_tokens > INT32_MAX - 1 || total_tokens * H >= UINT32_MAX)
+    // (The kernels find their work by walking over the sequences, inside the time of their bounded waits.)
+    if (n_seq > int64_t{1} << 22) return set_error(RHZ_ERR_SHAPE, "n_seq = %lld: at most 2^22 sequences", (long long)n_seq);
+    if (total_tokens > INT32_MAX - 1 || total_tokens * H >= UINT32_MAX)
         return set_error(RHZ_ERR_SHAPE, "n_seq = %lld, total_tokens = %lld: beyond int32 indexing", (long long)n_seq, (long long)total_tokens);
     return RHZ_OK;
 }

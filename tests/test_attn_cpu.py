@@ -171,3 +171,9 @@ def test_plain_trees_and_tables():
         [1, 1, 1, 0, 0, 1, 0, 1]]
     got = step_tables([3, 8], [6, 1], [[50, 0], [51, 0]], [1, 1], [7], 8, 8)
     assert got == ([0, 6, 7], [403, 404, 405, 406, 407, 56, -1, -1], [[50, 7], [51, 0]], [2, 1], 1, 1)
+
+
+def test_attention_refuses_more_sequences_than_its_walk_over_them_allows(lib):
+    for n, want in ((1 << 22, capi.RHZ_OK), ((1 << 22) + 1, capi.RHZ_ERR_SHAPE)):
+        assert lib.rhz_attn_varlen_fwd(*[FAKE] * 6, n, 0, 256, 128, 128, 8, 4, 32, 0.5, BF16, None) == want
+        assert lib.rhz_attn_tree_fwd(*[FAKE] * 9, n, 0, 8, 256, 4, 10, 16, 8, 4, 32, 0.5, BF16, None, 0, None) == want
