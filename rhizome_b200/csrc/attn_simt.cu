@@ -59,40 +59,31 @@ struct Found {
     int32_t seq, block, chunk;
 };
 
-// Unit x of the batch, units ordered (sequence, block, chunk); seq -1 past
-// the last. The CTA scans the sequences' unit counts in steps of its threads.
-__device__ Found find_unit(const AttnArgs &a, int64_t x, int tok, Split split) {
-    __shared__ int64_t sums[THREADS / 32];
+// Unit x of the batch, `most` to a block; seq -1 where there is none. Block j of
+// a sequence whose first row is f has number f / tok + i + j, i the sequence's
+// index: rounding f down loses less than the one block that i adds, so no two
+// blocks meet and the numbers stay below total / tok + n_seq. The CTA finds i by
+// a search that divides the sequences by its threads in each step. (Walking over
+// them all instead, every CTA took as long as there are sequences: 65,536 f32
+// prompts of one token, 2 heads of 32 channels, 22.1 ms against 2.5.)
+__device__ Found find_unit(const AttnArgs &a, int x, int tok, Split split, int most) {
     __shared__ Found found;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) found = {-1, 0, 0};
-    int64_t before = 0;
-    for (int64_t base = 0; base < a.n_seq; base += THREADS) {
-        const int64_t i = base + threadIdx.x;
-        int64_t units = 0, chunks = 1;
-        if (i < a.n_seq) {
-            const Seq s = seq_of(a, i);
-            if (a.paged) chunks = split.chunks(s.keys);
-            units = (static_cast<int64_t>(s.m) + tok - 1) / tok * chunks;
-        }
-        int64_t incl = units;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, incl, off);
-            if (lane >= off) incl += y;
-        }
-        __syncthreads();
-        if (lane == 31) sums[warp] = incl;
-        __syncthreads();
-        int64_t at = before + incl - units;
-        for (int w = 0; w < THREADS / 32; ++w) {
-            if (w < warp) at += sums[w];
-            before += sums[w];
-        }
-        if (x >= at && x < at + units)
-            found = {static_cast<int32_t>(i), static_cast<int32_t>((x - at) / chunks),
-                     static_cast<int32_t>((x - at) % chunks)};
-        if (x < before) break;
+    const int unit = x / most;
+    auto number = [&](int i) { return seq_of(a, i).first / tok + i; };  // (the launch refuses more than 31 bits count)
+    int lo = 0, hi = static_cast<int>(a.n_seq);  // number(lo) <= unit once a step is done
+    do {
+        const int step = (hi - lo + THREADS - 1) / THREADS;
+        const int i = lo + static_cast<int>(threadIdx.x) * step;
+        const int below = __syncthreads_count(i < hi && number(i) <= unit);
+        if (below == 0) return {-1, 0, 0};
+        lo += (below - 1) * step;
+        hi = min(hi, lo + step);
+    } while (hi - lo > 1);
+    if (threadIdx.x == 0) {
+        const Seq s = seq_of(a, lo);
+        const int block = unit - number(lo), chunk = x - unit * most;
+        const bool there = static_cast<int64_t>(block) * tok < s.m && chunk < (a.paged ? split.chunks(s.keys) : 1);
+        found = there ? Found{lo, block, chunk} : Found{-1, 0, 0};
     }
     __syncthreads();
     return found;
@@ -114,7 +105,7 @@ __global__ void __launch_bounds__(THREADS) attn_simt_kernel(const AttnArgs a, co
     float *sq = reinterpret_cast<float *>(smem4), *sk = sq + ROWS * ld, *sv = sk + KEYS * ld,
           *sp = sv + KEYS * d;
     const int G = a.H / a.Hkv, tok = ROWS / G, kvh = blockIdx.y;
-    const Found f = find_unit(a, blockIdx.x, tok, split);
+    const Found f = find_unit(a, blockIdx.x, tok, split, parts.most);
     if (f.seq < 0) return;
     const Seq s = seq_of(a, f.seq);
     const int64_t t0 = static_cast<int64_t>(f.block) * tok;
