@@ -474,8 +474,7 @@ int rhz_attn_varlen_fwd(void *o, float *lse, const void *q, const void *k, const
  * [0, num_blocks) are seen by nobody. Rows outside [cu_seqlens[0],
  * cu_seqlens[n_seq]) are left as they were. The key axis of a sequence is
  * computed in chunks chosen by its own length and joined in order, so results
- * do not depend on the batch (but a call of more than 4096 sequences takes
- * another form for few rows, with other roundings); `workspace` holds
+ * do not depend on the batch; `workspace` holds
  * rhz_attn_tree_workspace_bytes(...) bytes (256-byte aligned; NULL/0 when
  * that is 0); calls that share a workspace must not overlap on the GPU.
  */

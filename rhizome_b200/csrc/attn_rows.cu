@@ -32,7 +32,7 @@ using namespace attn;
 constexpr int WARPS = 4;
 constexpr int KEYS = 32;         // keys of a tile
 constexpr int STAGES = 3;        // tiles in a warp's ring
-constexpr int MAX_SEQ = 4096;    // sequences whose chunk counts fit in shared memory
+constexpr int MAX_SEQ = 4096;    // sequences of a launch: their chunk counts fit in shared memory
 
 // Sticky: a bounded wait of this kernel ran out.
 __device__ int g_rows_timeout;
@@ -495,12 +495,20 @@ int launch_t(const AttnArgs &a, const Parts &parts, Split split) {
 // One 16-row tile: with two, 74 sequences of 8,192 keys and 32 rows took 1,088 us
 // here and 552 us as a row tile of the tcgen05 form.
 bool attn_rows_supports(const AttnArgs &a) {
-    return a.paged && a.dtype == RHZ_DTYPE_BF16 && (a.d == 64 || a.d == 128) && a.n_seq <= MAX_SEQ &&
-           a.most * (a.H / a.Hkv) <= 16;
+    return a.paged && a.dtype == RHZ_DTYPE_BF16 && (a.d == 64 || a.d == 128) && a.most * (a.H / a.Hkv) <= 16;
 }
 
 int launch_attn_rows(const AttnArgs &a, const Parts &parts, Split split) {
-    return a.d == 128 ? launch_t<128>(a, parts, split) : launch_t<64>(a, parts, split);
+    int st = RHZ_OK;
+    for (int64_t from = 0; st == RHZ_OK && from < a.n_seq; from += MAX_SEQ) {  // rows, parents and partial results go by token
+        AttnArgs g = a;
+        g.n_seq = a.n_seq - from < MAX_SEQ ? a.n_seq - from : MAX_SEQ;
+        g.cu_seqlens += from;
+        g.cached += from;
+        g.block_table += from * a.width;
+        st = a.d == 128 ? launch_t<128>(g, parts, split) : launch_t<64>(g, parts, split);
+    }
+    return st;
 }
 
 int attn_rows_status(int *flag, bool clear) {

@@ -74,3 +74,27 @@ def test_f32_batches_of_very_many_short_sequences(paged):
         if not paged:
             whole = ops.attn_varlen_fwd(q, k, v, cu[a:b + 1].contiguous())
             assert torch.equal(whole[rows], o[rows]), (a, b)
+
+
+@pytest.mark.parametrize("d,nodes", [(128, 1), (64, 3)])
+def test_few_rows_of_more_sequences_than_one_launch_holds(d, nodes):
+    """The same form whatever the number of sequences: the same bits as calls
+    with fewer of them, on both sides of the launches' borders."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n, page = 9000, 16
+    width = 1600 // page
+    counts = torch.randint(0, nodes + 1, (n,), generator=torch.Generator().manual_seed(4))
+    at = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)])
+    total = int(at[-1])
+    cu = at.to(torch.int32).cuda()
+    q = torch.randn(total, 8, d, generator=g, device="cuda").to(BF)
+    kc, vc = (torch.randn(500, 2, page, d, generator=g, device="cuda").to(BF) for _ in range(2))
+    table = torch.randint(0, 500, (n, width), generator=g, device="cuda", dtype=torch.int32)
+    cached = torch.randint(0, 1500, (n,), generator=g, device="cuda", dtype=torch.int32)
+    parent = None if nodes == 1 else torch.randint(-1, 1, (total,), generator=g, device="cuda", dtype=torch.int32)
+    o, lse = ops.attn_tree_fwd(q, kc, vc, table, cached, cu, nodes, parent=parent, with_lse=True)
+    for a, b in ((0, 4), (4090, 4100), (4096, 4200), (8190, 8195), (n - 5, n)):
+        rows = slice(int(at[a]), int(at[b]))
+        part = ops.attn_tree_fwd(q[rows], kc, vc, table[a:b], cached[a:b], (cu[a:b + 1] - cu[a]).contiguous(), nodes,
+                                 parent=None if parent is None else parent[rows], with_lse=True)
+        assert torch.equal(part[0], o[rows]) and torch.equal(part[1], lse[rows]), (a, b)
