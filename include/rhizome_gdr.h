@@ -476,7 +476,10 @@ int rhz_attn_varlen_fwd(void *o, float *lse, const void *q, const void *k, const
  * computed in chunks chosen by its own length and joined in order, so results
  * do not depend on the batch; `workspace` holds
  * rhz_attn_tree_workspace_bytes(...) bytes (256-byte aligned; NULL/0 when
- * that is 0); calls that share a workspace must not overlap on the GPU.
+ * that is 0): for the table's width, total_tokens x H x (d + 1) x 4 bytes per
+ * chunk, up to 64 chunks (of 512 keys, 2,560 or 256 at least, by form) and with
+ * a bound above 64 fewer, down to four. Calls that share a workspace must not
+ * overlap on the GPU.
  */
 int rhz_attn_tree_fwd(void *o, float *lse, const void *q, const void *k_cache,
                       const void *v_cache, const int32_t *block_table, const int32_t *cached,

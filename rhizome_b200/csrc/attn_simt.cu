@@ -23,7 +23,7 @@ using namespace attn;
 
 constexpr int THREADS = 256;
 constexpr int KEYS = 64;                       // keys per tile
-constexpr Split SIMT_SPLIT{256, 64}, ROWS_SPLIT{512, 64};
+constexpr Split ROWS_SPLIT{512, 64};
 // Keys per chunk and chunks at most on the tcgen05 form (64 at most: the join
 // has two per lane). A unit costs some 3 us beside its keys, and its rows' partial
 // results are written and read again, so chunks are as long as an even deal
@@ -31,9 +31,32 @@ constexpr Split SIMT_SPLIT{256, 64}, ROWS_SPLIT{512, 64};
 // 706 of 4,096 and 612 of 8,192, but 48 trees over U{1..8192} keys 232, 238
 // and 316. The bound gives one long sequence two units per SM (131,072 keys and
 // 24 nodes: 112 us in 37 chunks, 141 in 32).
+//
+// A bound of more rows than a tree has (pieces of a prompt) lowers the most
+// chunks by the row blocks that a sequence can have, to four: the blocks fill
+// the SMs themselves, and the scratch, which the most chunks of the table's
+// width size, was 5 GB for 8,192 rows of 32 heads over 131,072 positions (0.5 GB
+// in four chunks, 21.2 -> 17.8 ms; 2,048 rows over 65,536 keys 2.9 -> 2.4 ms). What
+// it costs is a lone row in such a call: over 131,000 keys 437 us, not 134.
+int chunks_beside(int64_t blocks, int wanted, int most) {
+    const int64_t few = wanted / blocks;
+    const int least = most < 4 ? most : 4;
+    return few < least ? least : few < most ? static_cast<int>(few) : most;
+}
+
 Split tc_split(const AttnArgs &a) {
-    const int most = 2 * 148 / a.Hkv;
-    return {2560, most < 1 ? 1 : most < 64 ? most : 64};
+    int most = 2 * 148 / a.Hkv;
+    most = most < 1 ? 1 : most < 64 ? most : 64;
+    const int pair = 2 * (128 / (a.H / a.Hkv));  // tokens of a unit
+    if (a.most > MAX_NODES) most = chunks_beside((a.most + pair - 1) / pair, most, most);
+    return {2560, most};
+}
+
+// 16 or 64 rows to a CTA; some four of 64 to an SM.
+Split simt_split(const AttnArgs &a) {
+    const int tok = 64 / (a.H / a.Hkv);
+    const int most = a.most > MAX_NODES ? chunks_beside((a.most + tok - 1) / tok * a.Hkv, 4 * 148, 64) : 64;
+    return {256, most};
 }
 
 // Four consecutive elements as f32 (d % 4 == 0, 16-byte aligned bases).
@@ -415,7 +438,7 @@ int launch_simt(const AttnArgs &a, const Parts &parts, Split split) {
 }
 
 Split split_of(const AttnArgs &a) {
-    return attn_rows_supports(a) ? ROWS_SPLIT : attn_tc_supports(a) ? tc_split(a) : SIMT_SPLIT;
+    return attn_rows_supports(a) ? ROWS_SPLIT : attn_tc_supports(a) ? tc_split(a) : simt_split(a);
 }
 
 int64_t chunk_bound(const AttnArgs &a) {

@@ -177,3 +177,20 @@ def test_attention_refuses_more_sequences_than_its_walk_over_them_allows(lib):
     for n, want in ((1 << 22, capi.RHZ_OK), ((1 << 22) + 1, capi.RHZ_ERR_SHAPE)):
         assert lib.rhz_attn_varlen_fwd(*[FAKE] * 6, n, 0, 256, 128, 128, 8, 4, 32, 0.5, BF16, None) == want
         assert lib.rhz_attn_tree_fwd(*[FAKE] * 9, n, 0, 8, 256, 4, 10, 16, 8, 4, 32, 0.5, BF16, None, 0, None) == want
+
+
+def test_scratch_of_prompt_pieces_is_bounded_by_their_outputs(lib):
+    """A bound of rows beyond a tree's fills the card by itself: four chunks of
+    keys at most, whatever the table's width, once the row blocks do."""
+    w = lib.rhz_attn_tree_workspace_bytes
+    for tokens, width, page, H, Hkv, d, dt in ((8192, 8192, 16, 32, 8, 128, BF16), (65536, 10240, 16, 32, 4, 128, BF16),
+                                               (8192, 1 << 20, 16, 32, 8, 128, F32), (4096, 4096, 64, 64, 64, 96, BF16),
+                                               (8192, 1 << 17, 1024, 16, 1, 64, BF16)):
+        chunk = tokens * H * (d + 1) * 4
+        assert chunk < w(tokens, tokens, width, page, H, Hkv, d, dt) <= 4 * chunk + (1 << 20), (tokens, H, d)
+    # trees (up to 64 nodes) keep theirs, and a bound just above comes down from it in steps
+    tree = w(512, 64, 8192, 16, 32, 8, 128, BF16)
+    assert tree > 30 * 512 * 32 * 129 * 4
+    sizes = [w(512, most, 8192, 16, 32, 8, 128, BF16) for most in (64, 65, 128, 129, 256, 512, 4096)]
+    assert sizes == sorted(sizes, reverse=True) and sizes[-1] <= 4 * 512 * 32 * 129 * 4 + (1 << 20)
+    assert w(512, 4096, 8192, 16, 300, 300, 128, BF16) == 0  # (150 K/V heads and more: one chunk as ever)
