@@ -1020,8 +1020,9 @@ int check_attn_heads(int32_t H, int32_t H_kv, int32_t d, int32_t dtype) {
 }
 
 int check_scale(float scale) {
-    if (!(scale > 0.f) || !(scale < INFINITY))
-        return set_error(RHZ_ERR_INVALID, "scale = %g: must be finite and positive", (double)scale);
+    // (The kernels take it times log2 e, which has to be finite too.)
+    if (!(scale > 0.f) || !(scale < 0x1p127f))
+        return set_error(RHZ_ERR_INVALID, "scale = %g: must be positive and below 2^127", (double)scale);
     return RHZ_OK;
 }
 

@@ -194,3 +194,9 @@ def test_scratch_of_prompt_pieces_is_bounded_by_their_outputs(lib):
     sizes = [w(512, most, 8192, 16, 32, 8, 128, BF16) for most in (64, 65, 128, 129, 256, 512, 4096)]
     assert sizes == sorted(sizes, reverse=True) and sizes[-1] <= 4 * 512 * 32 * 129 * 4 + (1 << 20)
     assert w(512, 4096, 8192, 16, 300, 300, 128, BF16) == 0  # (150 K/V heads and more: one chunk as ever)
+
+
+def test_attention_refuses_a_scale_whose_product_with_log2_e_overflows(lib):
+    for scale, want in ((3e38, capi.RHZ_ERR_INVALID), (2.0 ** 127, capi.RHZ_ERR_INVALID), (2.0 ** 126, capi.RHZ_OK), (1e-40, capi.RHZ_OK)):
+        assert lib.rhz_attn_varlen_fwd(*[FAKE] * 6, 0, 0, 256, 128, 128, 8, 4, 32, scale, BF16, None) == want
+        assert lib.rhz_attn_tree_fwd(*[FAKE] * 9, 0, 0, 8, 256, 4, 10, 16, 8, 4, 32, scale, BF16, None, 0, None) == want
