@@ -130,10 +130,10 @@ def _call_on(dev: torch.device, name: str, *args) -> None:
             capi.call(name, *args, _stream(dev))
 
 
-def _same_device(dev: torch.device, *tensors):
-    for x in tensors:
+def _same_device(dev: torch.device, **tensors):
+    for name, x in tensors.items():
         if x is not None and x.device != dev:
-            raise capi.InvalidArgument(capi.RHZ_ERR_INVALID, f"a tensor is on {x.device}, others are on {dev}")
+            raise capi.InvalidArgument(capi.RHZ_ERR_INVALID, f"{name} is on {x.device}, expected {dev}")
 
 
 def _rows(x: torch.Tensor, name: str, dtype, tokens: int, H: int, d: int) -> int:
@@ -195,7 +195,8 @@ def gdr_tree_step(q, k, v, alpha, beta, cu_seqlens, parent, max_positions, state
     if states is not None:
         _need(states, "states", torch.float32, (tokens, H, d, d))
     dev = q.device
-    _same_device(dev, k, v, alpha, beta, cu_seqlens, parent, state_pool, slot_idx, out, states)
+    _same_device(dev, k=k, v=v, alpha=alpha, beta=beta, cu_seqlens=cu_seqlens, parent=parent,
+                 state_pool=state_pool, slot_idx=slot_idx, out=out, states=states)
     o = torch.empty_like(q) if out is None else out
     if states is None:
         states = torch.empty((tokens, H, d, d), device=dev, dtype=torch.float32)
@@ -228,7 +229,8 @@ def kv_step_tables(cached, fresh, block_table, held, free_blocks, page, max_toke
     if max_tokens < 0:
         raise capi.ShapeError(capi.RHZ_ERR_SHAPE, f"max_tokens = {max_tokens}: must be >= 0")
     dev = cached.device
-    _same_device(dev, fresh, held, block_table, free_blocks, cursor)
+    _same_device(dev, fresh=fresh, held=held, block_table=block_table, free_blocks=free_blocks,
+                 cursor=cursor)
     out = torch.empty(2 * n + 3, device=dev, dtype=torch.int32)
     cu, held_out, cursor_out, missing = torch.split_with_sizes(out, (n + 1, n, 1, 1))
     slot_map = torch.empty(max_tokens, device=dev, dtype=torch.int64)
@@ -256,7 +258,7 @@ def kv_append(k, v, slot_map, k_cache, v_cache):
     ks, vs = _rows(k, "k", k.dtype, tokens, H, d), _rows(v, "v", k.dtype, tokens, H, d)
     _need(slot_map, "slot_map", torch.int64, (tokens,))
     dev = k.device
-    _same_device(dev, v, slot_map, k_cache, v_cache)
+    _same_device(dev, v=v, slot_map=slot_map, k_cache=k_cache, v_cache=v_cache)
     _call_on(dev, "rhz_kv_append", _p(k_cache), _p(v_cache), _p(k), _p(v), _p(slot_map), tokens, ks,
              vs, num_blocks, page, H, d, _dt(k))
     return k_cache, v_cache
@@ -276,7 +278,7 @@ def attn_varlen_fwd(q, k, v, cu_seqlens, scale=None, out=None, with_lse=False):
     if out is not None:
         _need(out, "out", q.dtype, (tokens, H, d))
     dev = q.device
-    _same_device(dev, k, v, cu_seqlens, out)
+    _same_device(dev, k=k, v=v, cu_seqlens=cu_seqlens, out=out)
     o = torch.empty((tokens, H, d), device=dev, dtype=q.dtype) if out is None else out
     lse = torch.empty((tokens, H), device=dev, dtype=torch.float32) if with_lse else None
     _call_on(dev, "rhz_attn_varlen_fwd", _p(o), _p(lse), _p(q), _p(k), _p(v), _p(cu_seqlens), n,
@@ -315,7 +317,8 @@ def attn_tree_fwd(q, k_cache, v_cache, block_table, cached, cu_seqlens, max_posi
     if out is not None:
         _need(out, "out", q.dtype, (tokens, H, d))
     dev = q.device
-    _same_device(dev, k_cache, v_cache, block_table, cached, cu_seqlens, parent, out)
+    _same_device(dev, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cached=cached,
+                 cu_seqlens=cu_seqlens, parent=parent, out=out)
     width = block_table.shape[1]
     o = torch.empty((tokens, H, d), device=dev, dtype=q.dtype) if out is None else out
     lse = torch.empty((tokens, H), device=dev, dtype=torch.float32) if with_lse else None

@@ -200,3 +200,10 @@ def test_attention_refuses_a_scale_whose_product_with_log2_e_overflows(lib):
     for scale, want in ((3e38, capi.RHZ_ERR_INVALID), (2.0 ** 127, capi.RHZ_ERR_INVALID), (2.0 ** 126, capi.RHZ_OK), (1e-40, capi.RHZ_OK)):
         assert lib.rhz_attn_varlen_fwd(*[FAKE] * 6, 0, 0, 256, 128, 128, 8, 4, 32, scale, BF16, None) == want
         assert lib.rhz_attn_tree_fwd(*[FAKE] * 9, 0, 0, 8, 256, 4, 10, 16, 8, 4, 32, scale, BF16, None, 0, None) == want
+
+
+def test_a_tensor_on_another_device_is_named():
+    dev = torch.device("cpu")
+    ops._same_device(dev, k=torch.zeros(1), parent=None)
+    with pytest.raises(capi.InvalidArgument, match="v_cache is on meta, expected cpu"):
+        ops._same_device(dev, k_cache=torch.zeros(1), v_cache=torch.zeros(1, device="meta"))
