@@ -55,7 +55,7 @@ __device__ __forceinline__ int64_t scan_exclusive(int64_t x, int64_t *sums, int6
 // list where it is new, so no CTA reads what another writes.
 __global__ void __launch_bounds__(TABLE_THREADS) kv_tables_kernel(const KvTablesArgs a, int shift) {
     __shared__ int64_t s_sums[TABLE_THREADS / 32];
-    __shared__ int64_t s_row[TABLE_THREADS + 1];   // first slot-map row of each request of the step
+    __shared__ int64_t s_row[TABLE_THREADS];       // first slot-map row of each request of the step
     __shared__ int64_t s_off[TABLE_THREADS];       // its free-list offset
     __shared__ int32_t s_cached[TABLE_THREADS], s_held[TABLE_THREADS], s_now[TABLE_THREADS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -80,7 +80,6 @@ __global__ void __launch_bounds__(TABLE_THREADS) kv_tables_kernel(const KvTables
         s_cached[tid] = static_cast<int32_t>(cached);
         s_held[tid] = static_cast<int32_t>(held);
         s_now[tid] = static_cast<int32_t>(held + granted);
-        if (tid == 0) s_row[TABLE_THREADS] = rows + total_rows;
         if (blockIdx.x == 0) {
             if (in) {
                 a.cu_seqlens[i] = static_cast<int32_t>(row);
