@@ -10,7 +10,7 @@
 // row of the group shares each K and V byte), the softmax stays in registers.
 // Four warps with 48 KB in flight each keep an SM's share of HBM busy (44 KB
 // would cover one microsecond of it). 512 sequences of U{1..8192} keys, one
-// token, 16 heads over 4, pages of 16: 1,350 us, 6.2 TB/s, 0.95 of a plain copy's
+// token, 32 heads over 8, pages of 16: 1,350 us, 6.2 TB/s, 0.95 of a plain copy's
 // rate, and 26 us to join the chunks; 74 sequences of 8,192 keys and four tokens: 448 us,
 // 5.5 TB/s (rows of masked nodes and one round of units more for some SMs).
 #include <cuda.h>

@@ -24,14 +24,7 @@ using namespace attn;
 constexpr int THREADS = 256;
 constexpr int KEYS = 64;                       // keys per tile
 constexpr Split ROWS_SPLIT{512, 64};
-// Keys per chunk and chunks at most on the tcgen05 form (64 at most: the join
-// has two per lane). A unit costs some 3 us beside its keys, and its rows' partial
-// results are written and read again, so chunks are as long as an even deal
-// allows: 74 trees of 64 nodes over 8,192 keys took 768 us in chunks of 2,048,
-// 706 of 4,096 and 612 of 8,192, but 48 trees over U{1..8192} keys 232, 238
-// and 316. The bound gives one long sequence two units per SM (131,072 keys and
-// 24 nodes: 112 us in 37 chunks, 141 in 32).
-//
+
 // A bound of more rows than a tree has (pieces of a prompt) lowers the most
 // chunks by the row blocks that a sequence can have, to four: the blocks fill
 // the SMs themselves, and the scratch, which the most chunks of the table's
@@ -44,6 +37,13 @@ int chunks_beside(int64_t blocks, int wanted, int most) {
     return few < least ? least : few < most ? static_cast<int>(few) : most;
 }
 
+// Keys per chunk and chunks at most on the tcgen05 form (64 at most: the join
+// has two per lane). A unit costs some 3 us beside its keys, and its rows' partial
+// results are written and read again, so chunks are as long as an even deal
+// allows: 74 trees of 64 nodes over 8,192 keys took 768 us in chunks of 2,048,
+// 706 of 4,096 and 612 of 8,192, but 48 trees over U{1..8192} keys 232, 238
+// and 316. The bound gives one long sequence two units per SM (131,072 keys and
+// 24 nodes: 112 us in 37 chunks, 141 in 32).
 Split tc_split(const AttnArgs &a) {
     int most = 2 * 148 / a.Hkv;
     most = most < 1 ? 1 : most < 64 ? most : 64;
@@ -52,7 +52,8 @@ Split tc_split(const AttnArgs &a) {
     return {2560, most};
 }
 
-// 16 or 64 rows to a CTA; some four of 64 to an SM.
+// The rule counts blocks of 64 rows, four to an SM, also where 16 go to a CTA, so
+// that the bits are the same.
 Split simt_split(const AttnArgs &a) {
     const int tok = 64 / (a.H / a.Hkv);
     const int most = a.most > MAX_NODES ? chunks_beside((a.most + tok - 1) / tok * a.Hkv, 4 * 148, 64) : 64;

@@ -10,8 +10,8 @@
 //   O_x += P_x V             (tcgen05, P as a bf16 A operand in TMEM, over S's columns)
 // P is rounded to bf16 because the product takes one type, the type of V; its
 // sum is taken in f32 before the rounding. The maximum m is kept lazily: it is
-// looked for only when a step's sum says that it may have been left behind,
-// and O is rescaled only when it has grown by more than 2^8.
+// looked for only when a step's sum exceeds 2^16 (so the one in use may lag by as
+// much), and then O is rescaled only if it has grown by more than 2^8.
 //
 // Roles: warps 0-3 and 4-7 the softmax of tiles 0 and 1, warps 8 and 9 the
 // products of a tile each, warp 10 copies Q and K, warp 11 resolves units ahead
@@ -19,19 +19,24 @@
 // PV_x(e), QK_x(e + 2) lets the tensor cores work on one step while the softmax
 // is on another, and S_x(e + 2) complete implies PV_x(e) complete.
 //
-// What bounds it, of a step of 2 x 128 x 64 products at d = 128: the exponentials
-// take the SM's 16 special-function lanes 1,024 cycles, the products 896 of the
-// tensor cores (512 for PV, 384 for QK: 51 cycles each, not 32, as both operands
-// come from shared memory), and the softmax's instructions beside the
-// exponentials share its four schedulers. One prompt of 32,768 tokens (16 heads
-// over 4): 7.8 ms, 1.13 PFLOP/s, 0.70 of a large library product; tensor pipe
-// 75% busy. Steps of 64 keys with P and S held twice took 8.16 ms where steps of
-// 128 took 8.73, an issuing thread per tile and operands in uniform registers
-// 7.86. Measured and not kept, on the 128-key form: part of the exponentials
-// as polynomials on the FMA pipe (9.06 -> 9.30 ms and more with the share), the two tiles
-// taking turns at the exponentials (8.73 -> 8.80 ms).
-// Over the cache with one row tile it is the copies: 4.8 TB/s at 74 sequences
-// of 8,192 keys in pages of 16, where a box of 16 rows is issued every 60 cycles.
+// What bounds it: no one pipe, but the chain of scores, softmax, probabilities
+// and product of each row tile. Of a step of 2 x 128 x 64 products at d = 128 the
+// tensor pipe needs 1,024 cycles at its rate (8 PV products of 64 cycles, 16 QK of
+// 32; a QK product, both operands from shared memory, takes 51 alone and 36
+// between PV products, so 1,090 to 1,330), the exponentials 1,024 of the SM's 16
+// special-function lanes. A step takes 1,660 cycles in one prompt of 32,768 tokens
+// (both pipes 62% active) and 1,790 in 16 packed ones (57%); an instruction waits
+// 2.5 cycles for the one before it and 1.8 for memory, tensor memory mostly. One prompt
+// of 32,768 tokens (32 heads over 8): 7.2 ms in a launch of its own, 8.2 ms among
+// others under the power cap, 1.1 PFLOP/s, 0.66 of a large library product. Steps
+// of 64 keys with P and S held twice took 8.16 ms where steps of 128 took 8.73, an
+// issuing thread per tile and operands in uniform registers 7.86. Measured and
+// not kept, on the 128-key form: part of the exponentials as polynomials on the
+// FMA pipe (9.06 -> 9.30 ms and more with the share), the two tiles taking turns
+// at the exponentials (8.73 -> 8.80 ms).
+// Over the cache with one row tile only one of the softmax warpgroups works, 64
+// keys in 0.88 us per SM: 74 sequences of 8,192 keys and 32 rows 552 us, of which
+// reading them once is 379.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -54,7 +59,7 @@ constexpr int KEYS = 64;    // keys of a step
 constexpr int THREADS = 384;
 constexpr int WARP_MMA = 8, WARP_TMA = 10, WARP_SCHED = 11;  // (two of the first)
 constexpr int GROUP = 192;  // sequences whose unit counts the scheduler holds at a time
-constexpr float FREE = 65536.f;  // probabilities may reach this against a maximum that was not looked for
+constexpr float FREE = 65536.f;  // 2^16: probabilities may reach this against a maximum that was not looked for
 constexpr float LAZY = 8.f; // a row's maximum may grow by 2^LAZY before O is rescaled
 
 // Sticky: a bounded wait of this kernel ran out.
@@ -419,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     part[0] = add2(part[0], part[1]);
                 };
                 // Without looking for the maximum first: against the one in use
-                // no probability of these 64 is above 2^FREE if their sum is not
+                // no probability of these 64 is above FREE if their sum is not
                 // (the search took 280 of a step's 1,900 cycles).
                 bool settled = false;
                 if (e > 0 && !edge) {
