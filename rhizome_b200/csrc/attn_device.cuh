@@ -113,7 +113,8 @@ __device__ __forceinline__ uint32_t finite_word(uint32_t w) {
 // Values that are not finite at keys that not every row of a tile sees. The
 // tensor cores' 0 * NaN would take them to every row, so the kernels replace
 // them by zero in shared memory and, once a unit's rows are written, come here
-// for the keys [from, to) that this can be (128 of them and a step at most).
+// for the keys [from, to) that this can be (two row tiles' tokens, or a tree's
+// nodes, and a step at most).
 // What a row that sees such a key has to get follows without its probability:
 // that is positive, so an infinity stays one, and what was written is finite
 // there or not finite already. Only where the key's score is itself not finite
