@@ -410,8 +410,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             const int r = gq + 8 * i, t = r / g.group, of = r - t * g.group;
-            if (all[i] == 0 && bits[i] == 0) l = 0.f;  // sees nothing: whole tiles did not ask
-            some[i] = r < used && l != 0.f;
+            const bool none = all[i] == 0 && bits[i] == 0;
+            if (none) l = 0.f;  // sees nothing: whole tiles did not ask
+            // (Where every score is -inf the row is zeros, whatever 0 * inf left in the sums; a chunk keeps that for the join.)
+            some[i] = r < used && !none && (split || l != 0.f);
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const float l2 = l == 0.f ? -INFINITY : top[i] + log2f(l);
             if (r >= used) continue;
@@ -423,8 +425,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
                 float2 *dst = reinterpret_cast<float2 *>(g.parts.o + row * D + 2 * tq);
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n)
-                    dst[4 * n] = l == 0.f ? make_float2(0.f, 0.f)
-                                          : make_float2(acc[n][2 * i] * inv, acc[n][2 * i + 1] * inv);
+                    dst[4 * n] = none ? make_float2(0.f, 0.f) : make_float2(acc[n][2 * i] * inv, acc[n][2 * i + 1] * inv);
             } else {
                 if (tq == 0 && a.lse) a.lse[token * a.H + head] = l2 * LN2;
                 uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(a.o) + (token * a.H + head) * D + 2 * tq);

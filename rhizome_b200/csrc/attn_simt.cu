@@ -288,20 +288,24 @@ __global__ void __launch_bounds__(THREADS) attn_simt_kernel(const AttnArgs a, co
         const int head = kvh * G + r % G;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const float l2 = l == 0.f ? -INFINITY : top[i] + log2f(l);
+        auto result = [&](int g) {  // (zeros where every score is -inf, whatever 0 * inf left in the sums; a chunk keeps that for the join)
+            return l == 0.f && chunks == 1 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                           : make_float4(acc[i][g][0] * inv, acc[i][g][1] * inv, acc[i][g][2] * inv, acc[i][g][3] * inv);
+        };
         if (chunks > 1) {
             const int64_t row = parts.row(f.chunk, token, head);
             if (tx == 0) parts.lse[row] = l2;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const int c = 4 * (tx + 16 * g);
-                if (c < d) set4(parts.o + row * d + c, make_float4(acc[i][g][0] * inv, acc[i][g][1] * inv, acc[i][g][2] * inv, acc[i][g][3] * inv));
+                if (c < d) set4(parts.o + row * d + c, result(g));
             }
         } else {
             if (tx == 0 && a.lse) a.lse[token * a.H + head] = l2 * LN2;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const int c = 4 * (tx + 16 * g);
-                if (c < d) set4(static_cast<T *>(a.o) + (token * a.H + head) * d + c, make_float4(acc[i][g][0] * inv, acc[i][g][1] * inv, acc[i][g][2] * inv, acc[i][g][3] * inv));
+                if (c < d) set4(static_cast<T *>(a.o) + (token * a.H + head) * d + c, result(g));
             }
         }
         if (parts.count && tx == 0 && f.chunk == 0 && head == 0) parts.count[token] = static_cast<int32_t>(chunks);
@@ -371,7 +375,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, const 
         const int col = 4 * lane + 128 * g;
         if (col < a.d)
             set4(static_cast<T *>(a.o) + (token * a.H + head) * a.d + col,
-                 make_float4(acc[g][0] * inv, acc[g][1] * inv, acc[g][2] * inv, acc[g][3] * inv));
+                 total == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                              : make_float4(acc[g][0] * inv, acc[g][1] * inv, acc[g][2] * inv, acc[g][3] * inv));
     }
     if (lane == 0 && a.lse)
         a.lse[token * a.H + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;

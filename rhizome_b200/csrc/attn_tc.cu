@@ -506,7 +506,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             // each at a time, so that eight lanes write a row's whole line. The
             // loops stay rolled: this code runs once in a unit, and fetching
             // its instructions is most of its time.
-            const bool some = n > 0 && sees;
+            // (Where every score is -inf the row is zeros, whatever 0 * inf left in O; a chunk keeps that for the join.)
+            const bool some = n > 0 && sees && (split || sum != 0.f);
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const uint32_t mine = used && some ? static_cast<uint32_t>(split ? g.parts.row(0, row, head) : row * a.H + head) : ~0u;
             const uint32_t out = base + C::OFF_OUT + warp * 4096;
@@ -557,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     __syncwarp();
                 }
             }
-            if (used && !some) {  // a row that sees nothing
+            if (used && !some) {  // a row that sees nothing, or nothing but scores of -inf
                 uint32_t *z = reinterpret_cast<uint32_t *>(dst + (split ? g.parts.row(0, row, head) : row * a.H + head) * row_bytes);
 #pragma unroll 1
                 for (int c = 0; c < row_bytes / 4; ++c) z[c] = 0u;
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (PAGED && used && g.parts.count && u.chunk == 0 && head == 0) g.parts.count[row] = u.chunks;
             if (bad)
                 add_odd_values<D>(a, g.parts, {u.first, u.m, u.live, u.cached, u.keys}, {u.seq, u.kvh, u.chunk, u.chunks},
-                                  max(full_both(), kbeg), min(u.keys, kbeg + n * KEYS), used && sum != 0.f, token, head, lane);
+                                  max(full_both(), kbeg), min(u.keys, kbeg + n * KEYS), used && some, token, head, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(bars + 8 * (U_EMPTY + (i & 3)));

@@ -104,3 +104,26 @@ def spoil_last(c, q):
     (128, 1, [7000, 100], [300, 200], True), (64, 24, [9000], [20], False)])
 def test_split_keys_in_row_tiles(d, group, cached, counts, chain):
     check_tree(cached, counts, 2 * group, 2, d, BF, page=64, seed=group, chain=chain, change=spoil_nodes)
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 32), (F32, 200), (BF, 128), (BF, 64)])
+def test_rows_whose_scores_are_all_minus_infinity(dtype, d):
+    """0 / 0 by the formula: they are rows that see nothing (o = 0, lse = -inf),
+    whatever V holds there; the rows after them see finite scores too."""
+    def spoil(q, k, v, at):
+        q[:, :, 0] = q[:, :, 0].abs() + 0.5
+        for a, b in zip(at, at[1:]):
+            k[a:a + 3, :, 0] = -math.inf
+            v[a:a + 2, :, 1] = math.inf
+            v[a + 1:a + 3, :, 2] = math.nan
+    check_prompt([200, 3, 70], 4, 2, d, dtype, seed=1, spoil=spoil)
+
+    def change(c, q):
+        q[:, :, 0] = q[:, :, 0].abs() + 0.5
+        for k, v in zip(c.k, c.v):
+            k[:-2, :, 0] = -math.inf
+            v[5, :, 3] = math.inf
+            v[-3, :, 1] = math.nan
+    for nodes in (1, 3, 20):
+        check_tree([700, 6000, 10], [nodes] * 3, 4, 2, d, dtype, page=64, seed=nodes, change=change)
+        check_tree([700, 6000, 10], [nodes] * 3, 4, 2, d, dtype, page=64, seed=nodes, change=change, chain=True)
