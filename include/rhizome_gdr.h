@@ -446,8 +446,9 @@ int rhz_kv_append(void *k_cache, void *v_cache, const void *k, const void *v,
  * at most 2^22 sequences (empty ones count).
  * Rows outside [cu_seqlens[0], cu_seqlens[n_seq]) are left as they were.
  * Values of rows that a row does not see never reach it, NaN and infinities
- * included; a row whose scores are all -inf gives o = 0, lse = -inf. H a multiple of H_kv, at most 64 query heads to a K/V head; d a
- * multiple of 4 (8 for bf16), at most 256; scale positive, below 2^127.
+ * included; a row whose scores are all -inf gives o = 0, lse = -inf. H a
+ * multiple of H_kv, at most 64 query heads to a K/V head; d a multiple of 4 (8
+ * for bf16), at most 256; scale positive, below 2^127.
  * bf16 with d of 64 or 128 runs on the tensor cores (products of bf16 with
  * f32 sums, probabilities rounded to bf16), everything else in f32
  * arithmetic. Results do not depend on what else is in the batch.
